@@ -1,0 +1,435 @@
+// kv_select.hip — key bounds of page groups, selection of groups by a bound on their scores, eviction of groups by
+// accumulated weight (chromofold/kv_select.h).
+#include <algorithm>
+#include <cmath>
+
+#include "cf_device.hpp"
+#include "chromofold/kv_select.h"
+#include "kv_topk.hpp"
+
+namespace {
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kMaxGroups = 1u << 26;  // tables are shorter: 64 * max_groups fits 32 bits
+constexpr int kRows = 16;                  // query heads of one KV head an MFMA tile takes
+
+// Tokens of a sequence its query sees, and tokens its table can hold.
+__device__ __forceinline__ uint32_t visible_tokens(uint32_t tokens, uint32_t pos, uint32_t max_groups) {
+  if (tokens == 0) return 0;
+  return min(min(tokens - 1, pos), 64 * max_groups - 1) + 1;  // (pos + 1 could wrap)
+}
+
+// ---- key bounds -------------------------------------------------------------------------------------------------
+// One wavefront per group: a lane keeps 4 channels of every second (D = 128) or fourth (D = 64) token, 1 KiB per wavefront
+// load. Max, min and a finiteness test of 4 D 64 B per group: bound by the read.
+constexpr int kBoundWaves = 4;
+
+template <int D>
+__global__ __launch_bounds__(64 * kBoundWaves) void key_bounds_kernel(
+    const float *__restrict__ keys, uint64_t ngroups, const uint64_t *__restrict__ first_page,
+    const uint32_t *__restrict__ page_counts, const uint32_t *__restrict__ token_counts, const uint64_t *__restrict__ slots,
+    int8_t *__restrict__ codes, float *__restrict__ scales, uint64_t slot_count) {
+  constexpr int kL = D / 4;        // lanes of a token
+  constexpr int kT = 64 / kL;      // tokens of a wavefront load
+  constexpr int kIt = 16 / kT;     // loads of a page
+  const int lane = threadIdx.x & 63;
+  const uint64_t nw = static_cast<uint64_t>(gridDim.x) * kBoundWaves;
+  for (uint64_t g = static_cast<uint64_t>(blockIdx.x) * kBoundWaves + (threadIdx.x >> 6); g < ngroups; g += nw) {
+    const uint64_t slot = slots ? slots[g] : g;
+    if (slot >= slot_count) continue;
+    const uint32_t np = page_counts[g];
+    const uint64_t p0 = first_page[g];
+    float hi[4], lo[4], odd = 0.0f;  // odd: a NaN once a value was not finite
+#pragma unroll
+    for (int j = 0; j < 4; ++j) hi[j] = -INFINITY, lo[j] = -INFINITY;
+    bool bad = np == 0 || np > CF_KV_GROUP_PAGES;
+    uint32_t nt[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      nt[p] = bad || static_cast<uint32_t>(p) >= np ? 0u : token_counts ? token_counts[p0 + p] : 16u;
+      bad |= !bad && static_cast<uint32_t>(p) < np && (nt[p] == 0 || nt[p] > 16u);
+    }
+    if (!bad) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        if (static_cast<uint32_t>(p) >= np) break;
+        const float *page = keys + (p0 + p) * (16 * D);
+        float4_t x[kIt];
+#pragma unroll
+        for (int i = 0; i < kIt; ++i) x[i] = *reinterpret_cast<const float4_t *>(page + (i * 64 + lane) * 4);
+#pragma unroll
+        for (int i = 0; i < kIt; ++i)
+          if (static_cast<uint32_t>(i * kT + lane / kL) < nt[p]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              hi[j] = fmaxf(hi[j], x[i][j]);
+              lo[j] = fmaxf(lo[j], -x[i][j]);
+              odd = __builtin_fmaf(x[i][j], 0.0f, odd);
+            }
+          }
+      }
+    }
+#pragma unroll
+    for (int o = kL; o < 64; o <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        hi[j] = fmaxf(hi[j], __shfl_xor(hi[j], o));
+        lo[j] = fmaxf(lo[j], __shfl_xor(lo[j], o));
+      }
+    bad |= __builtin_amdgcn_ballot_w64(odd != odd) != 0;
+    float top = fmaxf(fmaxf(fmaxf(hi[0], lo[0]), fmaxf(hi[1], lo[1])), fmaxf(fmaxf(hi[2], lo[2]), fmaxf(hi[3], lo[3])));
+#pragma unroll
+    for (int o = 1; o < kL; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float s = bad ? INFINITY : top / 127.0f;
+    uint32_t ch = 0, cl = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // outward, so that the codes bound the keys; |x| <= top: at most 127 but for the quotient's rounding
+      const int a = bad ? 127 : s == 0.0f ? 0 : static_cast<int>(fmaxf(fminf(ceilf(hi[j] / s), 127.0f), -127.0f));
+      const int b = bad ? 127 : s == 0.0f ? 0 : static_cast<int>(fmaxf(fminf(ceilf(lo[j] / s), 127.0f), -127.0f));
+      ch |= (static_cast<uint32_t>(a) & 255u) << (8 * j);
+      cl |= (static_cast<uint32_t>(b) & 255u) << (8 * j);
+    }
+    if (lane < kL) {
+      uint32_t *rec = reinterpret_cast<uint32_t *>(codes + slot * (2 * D));
+      rec[lane] = ch;
+      rec[kL + lane] = cl;
+      if (lane == 0) scales[slot] = s;
+    }
+  }
+}
+
+// ---- selection --------------------------------------------------------------------------------------------------
+// Scores of 16 groups at a time on v_mfma_i32_16x16x64_i8: rows = the KV head's query heads, columns = groups, k = the 2 D
+// products of one group, [max(a, 0), max(-a, 0)] . [upper codes, negated lower codes]. A group's record is read by four
+// lanes in 16-byte pieces, every line of it whole within one step of the wavefront.
+template <int D>
+__device__ __forceinline__ void stage_query(const cf_kv_select_desc &d, uint32_t seq, uint32_t head, int8_t (*s_a)[2 * D],
+                                            float *s_step, int nthreads) {
+  const uint32_t gqa = d.query_head_count / d.kv_head_count;
+  const int lane = threadIdx.x & 63;
+  for (int h = threadIdx.x >> 6; h < kRows; h += nthreads >> 6) {  // a wavefront per query head
+    constexpr int kN = D / 64;
+    float q[kN], top = 0.0f;
+    const float *row = d.queries + (static_cast<size_t>(seq) * d.query_head_count + head * gqa + h) * D;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      q[j] = static_cast<uint32_t>(h) < gqa ? row[lane + 64 * j] : 0.0f;
+      top = fmaxf(top, fabsf(q[j]));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float step = top / 127.0f;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      const float r = q[j] / step;  // NaN for a NaN, for inf / inf and for 0 / 0: code 0
+      const int a = r == r ? static_cast<int>(fmaxf(fminf(rintf(r), 127.0f), -127.0f)) : 0;
+      s_a[h][lane + 64 * j] = static_cast<int8_t>(max(a, 0));
+      s_a[h][D + lane + 64 * j] = static_cast<int8_t>(max(-a, 0));
+    }
+    if (lane == 0) s_step[h] = step;
+  }
+}
+
+// Keys (sortable scores) of the units of tile `tile` (16 groups) of one (sequence, KV head) row; lane n of the first
+// sixteen returns its group's (unit 1) or its pair's (unit 2) key, 0 where nothing is visible.
+template <int D>
+__device__ __forceinline__ uint32_t score_tile(const int8_t *__restrict__ codes, const float *__restrict__ scales,
+                                               uint32_t tile, uint32_t ngroups, uint32_t unit, uint32_t gqa,
+                                               const int4_t *a, const float *step) {
+  const int lane = threadIdx.x & 63, n = lane & 15, kb = lane >> 4;
+  const uint32_t g = 16 * tile + n;
+  const size_t gc = min(g, ngroups - 1);
+  const int8_t *rec = codes + gc * (2 * D) + 16 * kb;
+  constexpr int kSteps = 2 * D / 64;
+  int4_t b[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) b[s] = *reinterpret_cast<const int4_t *>(rec + 64 * s);
+  const float scale = scales[gc];
+  int4_t c = {0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b[s], c, 0, 0, 0);
+  float best = -INFINITY;  // rows 4 kb .. 4 kb + 3; a head whose step is not finite gives a NaN, which fmaxf passes over
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (static_cast<uint32_t>(4 * kb + r) < gqa) best = fmaxf(best, static_cast<float>(c[r]) * step[r]);
+  best = cfd::rows4_max(best);
+  uint32_t key = g < ngroups ? cfsel::sortable(best * scale) : 0u;
+  if (unit == 2) key = max(key, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(key), 0xb1, 0xf, 0xf, false)));
+  return key;
+}
+
+template <int D>
+struct QueryOperand {
+  int4_t a[2 * D / 64];
+  float step[4];
+  __device__ __forceinline__ void load(const int8_t (*s_a)[2 * D], const float *s_step) {
+    const int lane = threadIdx.x & 63, n = lane & 15, kb = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < 2 * D / 64; ++s) a[s] = *reinterpret_cast<const int4_t *>(&s_a[n][64 * s + 16 * kb]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) step[r] = s_step[4 * kb + r];
+  }
+};
+
+constexpr int kScoreThreads = 256;
+
+// Scores to the workspace: grid (workgroups of a row, KV heads, sequences).
+template <int D>
+__global__ __launch_bounds__(kScoreThreads) void score_kernel(cf_kv_select_desc d, uint32_t *__restrict__ keys,
+                                                              uint32_t row_units) {
+  __shared__ __attribute__((aligned(16))) int8_t s_a[kRows][2 * D];
+  __shared__ float s_step[kRows];
+  const uint32_t head = blockIdx.y, seq = blockIdx.z, unit = d.unit_groups;
+  const uint32_t ngroups = (visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups) + 63) / 64;
+  const uint32_t tiles = (ngroups + 15) / 16, per = kScoreThreads / 64;
+  if (blockIdx.x * per >= tiles) return;
+  stage_query<D>(d, seq, head, s_a, s_step, kScoreThreads);
+  __syncthreads();
+  QueryOperand<D> q;
+  q.load(s_a, s_step);
+  const size_t row = static_cast<size_t>(seq) * d.kv_head_count + head;
+  const int8_t *codes = d.codes + row * d.max_groups * (2 * D);
+  const float *scales = d.scales + row * d.max_groups;
+  const int lane = threadIdx.x & 63;
+  for (uint32_t t = blockIdx.x * per + (threadIdx.x >> 6); t < tiles; t += gridDim.x * per) {
+    const uint32_t key = score_tile<D>(codes, scales, t, ngroups, unit, d.query_head_count / d.kv_head_count, q.a, q.step);
+    if (lane < 16 && lane % unit == 0) {
+      const uint32_t u = (16 * t + lane) / unit;
+      if (u < row_units) keys[row * row_units + u] = key;
+    }
+  }
+}
+
+constexpr int kPickThreads = 512;
+
+__device__ __forceinline__ void fill_none(uint32_t *p, uint32_t from, uint32_t to, int nthreads) {
+  for (uint32_t i = from + threadIdx.x; i < to; i += nthreads) p[i] = CF_KV_NO_UNIT;
+}
+
+template <int T, typename Keys>
+__device__ __forceinline__ void pick_units(const cf_kv_select_desc &d, size_t row, uint32_t n, const Keys &keys,
+                                           cfsel::TopkShared<T> &sh) {
+  uint32_t *out = d.units + row * d.max_units;
+  const uint32_t k = min(n, d.max_units);
+  cfsel::take_largest<T>([&](uint32_t i) { return keys[i]; }, n, d.keep_first, d.keep_last, k, sh,
+                         [&](uint32_t i, bool take, uint32_t pos) {
+                           if (take) out[pos] = i;
+                         },
+                         [](uint32_t, uint32_t, uint32_t) {});
+  fill_none(out, k, d.max_units, T);
+}
+
+// The best units of each row from the scores in the workspace: grid (KV heads, sequences).
+__global__ __launch_bounds__(kPickThreads) void pick_kernel(cf_kv_select_desc d, const uint32_t *__restrict__ keys,
+                                                            uint32_t row_units) {
+  __shared__ cfsel::TopkShared<kPickThreads> sh;
+  const uint32_t head = blockIdx.x, seq = blockIdx.y;
+  const uint32_t span = 64 * d.unit_groups;
+  const uint32_t vis = visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups);
+  const uint32_t n = vis / span + (vis % span != 0);
+  const size_t row = static_cast<size_t>(seq) * d.kv_head_count + head;
+  pick_units<kPickThreads>(d, row, n, keys + row * row_units, sh);
+}
+
+uint32_t row_units(const cf_kv_select_desc *d) { return (d->max_groups + d->unit_groups - 1) / d->unit_groups; }
+
+// ---- eviction ---------------------------------------------------------------------------------------------------
+constexpr int kEvictThreads = 256;
+
+struct Budget {
+  uint32_t tokens, groups, units, kept;
+  __device__ Budget(const cf_kv_evict_desc &d, uint32_t t) {
+    tokens = min(t, 64 * d.max_groups);
+    groups = tokens / 64 + (tokens % 64 != 0);
+    units = groups / d.unit_groups + (groups % d.unit_groups != 0);
+    kept = min(units, d.budget_units);
+  }
+  __device__ uint32_t tokens_out(const cf_kv_evict_desc &d) const { return tokens - 64 * d.unit_groups * (units - kept); }
+};
+
+__global__ void evict_tokens_kernel(cf_kv_evict_desc d) {
+  const uint32_t s = blockIdx.x * blockDim.x + threadIdx.x;
+  if (s < d.seq_count) d.seq_tokens_out[s] = Budget(d, d.seq_tokens[s]).tokens_out(d);
+}
+
+// One workgroup per (KV head, sequence). Units are decided and moved in rounds of kEvictThreads of them in index order: a
+// kept unit moves down or stays, so a round's destinations lie at or before its sources and before every later round's;
+// within a round all reads come before the first write. That is what makes eviction in place safe.
+template <int D>
+__global__ __launch_bounds__(kEvictThreads) void evict_kernel(cf_kv_evict_desc d, bool tokens_here) {
+  __shared__ cfsel::TopkShared<kEvictThreads> sh;
+  __shared__ uint32_t s_from[2 * kEvictThreads];  // source groups of the round's kept groups
+  const uint32_t head = blockIdx.x, seq = blockIdx.y, unit = d.unit_groups;
+  const uint32_t tid = threadIdx.x;
+  const Budget b(d, d.seq_tokens[seq]);
+  const size_t row = (static_cast<size_t>(seq) * d.kv_head_count + head) * d.max_groups;
+  const float *w = d.weights + row;
+  const uint32_t *off = d.group_offsets + row;
+  uint32_t *off_out = d.group_offsets_out + row;
+  auto wait_loads = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+
+  auto key = [&](uint32_t u) {
+    float x = w[u * unit];
+    if (unit == 2 && 2 * u + 1 < b.groups) x += w[2 * u + 1];
+    return cfsel::sortable(x);
+  };
+  cfsel::take_largest<kEvictThreads>(
+      key, b.units, d.keep_first, d.keep_last, b.kept, sh,
+      [&](uint32_t u, bool take, uint32_t pos) {
+        for (uint32_t j = 0; j < unit; ++j) {
+          const uint32_t g = u * unit + j;
+          if (take) {
+            if (g < b.groups) s_from[(pos * unit + j) % (2 * kEvictThreads)] = g;
+          } else if (d.dropped) {
+            d.dropped[row + pos * unit + j] = off[g];  // a dropped unit is not the last: all its groups exist
+          }
+        }
+      },
+      [&](uint32_t base, uint32_t before, uint32_t cnt) {
+        // kept groups [g0, g1) of the round; s_from is read at the same positions modulo its size
+        const uint32_t g0 = before * unit, g1 = min((before + cnt) * unit, b.groups - (b.units - b.kept) * unit);
+        __syncthreads();
+        for (uint32_t a = g0; a < g1; a += kEvictThreads) {  // (two steps for pairs)
+          const uint32_t i = a + tid;
+          const bool in = i < g1;
+          const uint32_t src = in ? s_from[i % (2 * kEvictThreads)] : 0u;
+          uint32_t o = 0;
+          float x = 0.0f, sc = 0.0f;
+          if (in) {
+            o = off[src];
+            if (d.weights_out) x = w[src];
+            if (d.codes_out) sc = d.scales[row + src];
+          }
+          wait_loads();
+          __syncthreads();
+          if (in) {
+            off_out[i] = o;
+            if (d.weights_out) d.weights_out[row + i] = x;
+            if (d.codes_out) d.scales_out[row + i] = sc;
+          }
+          if (d.codes_out) {
+            constexpr uint32_t kL = 2 * D / 16;  // 16-byte pieces of a record
+            constexpr uint32_t kPer = 8;         // pieces a thread moves at a time
+            const uint32_t m = min(g1 - a, static_cast<uint32_t>(kEvictThreads)) * kL;
+            for (uint32_t p0 = 0; p0 < m; p0 += kPer * kEvictThreads) {
+              int4_t v[kPer];
+#pragma unroll
+              for (uint32_t e = 0; e < kPer; ++e) {
+                const uint32_t p = p0 + e * kEvictThreads + tid;
+                if (p < m)
+                  v[e] = *reinterpret_cast<const int4_t *>(d.codes + (row + s_from[(a + p / kL) % (2 * kEvictThreads)]) * (2 * D) +
+                                                           16 * (p % kL));
+              }
+              wait_loads();
+              __syncthreads();
+#pragma unroll
+              for (uint32_t e = 0; e < kPer; ++e) {
+                const uint32_t p = p0 + e * kEvictThreads + tid;
+                if (p < m) *reinterpret_cast<int4_t *>(d.codes_out + (row + a + p / kL) * (2 * D) + 16 * (p % kL)) = v[e];
+              }
+            }
+          }
+        }
+        __syncthreads();  // s_from is free for the next round
+      });
+  const uint32_t left = b.groups - (b.units - b.kept) * unit, gone = b.groups - left;
+  __syncthreads();  // every weight has been read
+  if (d.weights_out)
+    for (uint32_t i = left + tid; i < d.max_groups; i += kEvictThreads) d.weights_out[row + i] = 0.0f;
+  if (d.dropped)
+    for (uint32_t i = gone + tid; i < d.max_groups; i += kEvictThreads) d.dropped[row + i] = CF_KV_NO_UNIT;
+  if (tokens_here && head == 0 && tid == 0) d.seq_tokens_out[seq] = b.tokens_out(d);
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// grids have the sequences or KV heads in y and z
+bool shape_ok(uint32_t seqs, uint32_t heads) { return seqs <= 65535 && heads <= 65535; }
+
+}  // namespace
+
+extern "C" cf_status cf_kv_key_bounds_async(const float *keys, uint64_t ngroups, const uint64_t *first_page,
+                                            const uint32_t *page_counts, const uint32_t *token_counts, uint32_t head_dim,
+                                            const uint64_t *slots, int8_t *codes, float *scales, uint64_t slot_count,
+                                            void *stream) {
+  if (!keys || !first_page || !page_counts || !codes || !scales || ngroups == 0) return CF_ERR_INVALID_ARGUMENT;
+  if (!aligned16(keys) || !aligned16(codes)) return CF_ERR_INVALID_ARGUMENT;
+  if (head_dim != 64 && head_dim != 128) return CF_ERR_UNSUPPORTED;
+  const uint64_t wg = (ngroups + kBoundWaves - 1) / kBoundWaves;
+  const dim3 grid(static_cast<uint32_t>(std::min<uint64_t>(wg, 1u << 20)));
+  const hipStream_t s = cfd::as_stream(stream);
+  if (head_dim == 128)
+    key_bounds_kernel<128><<<grid, 64 * kBoundWaves, 0, s>>>(keys, ngroups, first_page, page_counts, token_counts, slots,
+                                                             codes, scales, slot_count);
+  else
+    key_bounds_kernel<64><<<grid, 64 * kBoundWaves, 0, s>>>(keys, ngroups, first_page, page_counts, token_counts, slots,
+                                                            codes, scales, slot_count);
+  return cfd::launch_status();
+}
+
+extern "C" cf_status cf_kv_validate_select_desc(const cf_kv_select_desc *d) {
+  if (!d || d->struct_size != sizeof(cf_kv_select_desc) || d->abi_version != CF_KV_SELECT_ABI_VERSION)
+    return CF_ERR_INVALID_ARGUMENT;
+  if (!d->codes || !d->scales || !d->seq_tokens || !d->query_pos || !d->queries || !d->units || d->seq_count == 0 ||
+      d->kv_head_count == 0 || d->query_head_count == 0 || d->query_head_count % d->kv_head_count != 0 ||
+      d->max_groups == 0 || d->max_units == 0 || !aligned16(d->codes))
+    return CF_ERR_INVALID_ARGUMENT;
+  if (d->unit_groups != 1 && d->unit_groups != 2) return CF_ERR_INVALID_ARGUMENT;
+  if (d->keep_first > d->max_units || d->keep_last > d->max_units - d->keep_first) return CF_ERR_INVALID_ARGUMENT;
+  if (d->head_dim != 64 && d->head_dim != 128) return CF_ERR_UNSUPPORTED;
+  if (d->query_head_count / d->kv_head_count > CF_KV_SELECT_MAX_GQA) return CF_ERR_UNSUPPORTED;
+  if (!shape_ok(d->seq_count, d->kv_head_count) || d->max_groups >= kMaxGroups) return CF_ERR_UNSUPPORTED;
+  return CF_OK;
+}
+
+extern "C" uint64_t cf_kv_select_workspace_bytes(const cf_kv_select_desc *d) {
+  if (cf_kv_validate_select_desc(d) != CF_OK) return 0;
+  return static_cast<uint64_t>(d->seq_count) * d->kv_head_count * row_units(d) * sizeof(uint32_t);
+}
+
+extern "C" cf_status cf_kv_select_groups_async(const cf_kv_select_desc *d, void *stream) {
+  const cf_status v = cf_kv_validate_select_desc(d);
+  if (v != CF_OK) return v;
+  const uint64_t need = cf_kv_select_workspace_bytes(d);
+  if (need && (!d->workspace || d->workspace_bytes < need || !aligned16(d->workspace))) return CF_ERR_INVALID_ARGUMENT;
+  const hipStream_t s = cfd::as_stream(stream);
+  const uint32_t units = row_units(d);
+  uint32_t *keys = static_cast<uint32_t *>(d->workspace);
+  const uint32_t tiles = (d->max_groups + 15) / 16, per = kScoreThreads / 64;
+  const dim3 grid(std::min<uint32_t>((tiles + per - 1) / per, 1u << 16), d->kv_head_count, d->seq_count);
+  if (d->head_dim == 128) score_kernel<128><<<grid, kScoreThreads, 0, s>>>(*d, keys, units);
+  else score_kernel<64><<<grid, kScoreThreads, 0, s>>>(*d, keys, units);
+  pick_kernel<<<dim3(d->kv_head_count, d->seq_count), kPickThreads, 0, s>>>(*d, keys, units);
+  return cfd::launch_status();
+}
+
+extern "C" cf_status cf_kv_validate_evict_desc(const cf_kv_evict_desc *d) {
+  if (!d || d->struct_size != sizeof(cf_kv_evict_desc) || d->abi_version != CF_KV_SELECT_ABI_VERSION)
+    return CF_ERR_INVALID_ARGUMENT;
+  if (!d->group_offsets || !d->seq_tokens || !d->weights || !d->group_offsets_out || !d->seq_tokens_out ||
+      d->seq_count == 0 || d->kv_head_count == 0 || d->max_groups == 0 || d->budget_units == 0)
+    return CF_ERR_INVALID_ARGUMENT;
+  if (d->unit_groups != 1 && d->unit_groups != 2) return CF_ERR_INVALID_ARGUMENT;
+  if (d->keep_last == 0 || d->keep_first > d->budget_units || d->keep_last > d->budget_units - d->keep_first)
+    return CF_ERR_INVALID_ARGUMENT;
+  const int records = (d->codes != nullptr) + (d->scales != nullptr) + (d->codes_out != nullptr) + (d->scales_out != nullptr);
+  if ((records != 0 && records != 4) || !aligned16(d->codes) || !aligned16(d->codes_out)) return CF_ERR_INVALID_ARGUMENT;
+  if (d->head_dim != 64 && d->head_dim != 128) return CF_ERR_UNSUPPORTED;
+  if (!shape_ok(d->seq_count, d->kv_head_count) || d->max_groups >= kMaxGroups) return CF_ERR_UNSUPPORTED;
+  return CF_OK;
+}
+
+extern "C" cf_status cf_kv_evict_groups_async(const cf_kv_evict_desc *d, void *stream) {
+  const cf_status v = cf_kv_validate_evict_desc(d);
+  if (v != CF_OK) return v;
+  const hipStream_t s = cfd::as_stream(stream);
+  // in place, the lengths are still read by the workgroups of the other heads: a launch of their own behind them
+  const bool tokens_here = d->seq_tokens_out != d->seq_tokens;
+  const dim3 grid(d->kv_head_count, d->seq_count);
+  if (d->head_dim == 128) evict_kernel<128><<<grid, kEvictThreads, 0, s>>>(*d, tokens_here);
+  else evict_kernel<64><<<grid, kEvictThreads, 0, s>>>(*d, tokens_here);
+  if (!tokens_here) evict_tokens_kernel<<<cfd::grid_for(d->seq_count, 256), 256, 0, s>>>(*d);
+  return cfd::launch_status();
+}
