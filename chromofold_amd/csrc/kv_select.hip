@@ -2,6 +2,7 @@
 // accumulated weight (chromofold/kv_select.h).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "cf_device.hpp"
 #include "chromofold/kv_select.h"
@@ -52,24 +53,32 @@ __global__ __launch_bounds__(64 * kBoundWaves) void key_bounds_kernel(
       bad |= !bad && static_cast<uint32_t>(p) < np && (nt[p] == 0 || nt[p] > 16u);
     }
     if (!bad) {
+      float4_t x[4][kIt];  // the whole group in flight (absent pages: the last one again, no tokens of it)
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        if (static_cast<uint32_t>(p) >= np) break;
-        const float *page = keys + (p0 + p) * (16 * D);
-        float4_t x[kIt];
-#pragma unroll
-        for (int i = 0; i < kIt; ++i) x[i] = *reinterpret_cast<const float4_t *>(page + (i * 64 + lane) * 4);
+        const float *page = keys + (p0 + min(static_cast<uint32_t>(p), np - 1)) * (16 * D);
 #pragma unroll
         for (int i = 0; i < kIt; ++i)
-          if (static_cast<uint32_t>(i * kT + lane / kL) < nt[p]) {
+          x[p][i] = __builtin_nontemporal_load(reinterpret_cast<const float4_t *>(page + (i * 64 + lane) * 4));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      auto take = [&](auto masked) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < kIt; ++i) {
+            const bool here = !decltype(masked)::value || static_cast<uint32_t>(i * kT + lane / kL) < nt[p];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              hi[j] = fmaxf(hi[j], x[i][j]);
-              lo[j] = fmaxf(lo[j], -x[i][j]);
-              odd = __builtin_fmaf(x[i][j], 0.0f, odd);
+              const float v = x[p][i][j];
+              hi[j] = fmaxf(hi[j], here ? v : -INFINITY);
+              lo[j] = fmaxf(lo[j], here ? -v : -INFINITY);
+              odd = __builtin_fmaf(here ? v : 0.0f, 0.0f, odd);
             }
           }
-      }
+      };
+      if ((nt[0] & nt[1] & nt[2] & nt[3]) == 16u) take(std::false_type{});
+      else take(std::true_type{});
     }
 #pragma unroll
     for (int o = kL; o < 64; o <<= 1)
@@ -133,30 +142,59 @@ __device__ __forceinline__ void stage_query(const cf_kv_select_desc &d, uint32_t
   }
 }
 
-// Keys (sortable scores) of the units of tile `tile` (16 groups) of one (sequence, KV head) row; lane n of the first
-// sixteen returns its group's (unit 1) or its pair's (unit 2) key, 0 where nothing is visible.
+// Records of the 16 groups of a tile. Read as they lie, 1 KiB a wavefront load, and brought to the layout of a B operand
+// (lane (kb, n): quarters of group n) through LDS: loads in that layout touch 64 lines each, at which one CU's cache gives
+// 34 GB/s (2048 groups of a row 22 us, against 12 so).
 template <int D>
-__device__ __forceinline__ uint32_t score_tile(const int8_t *__restrict__ codes, const float *__restrict__ scales,
-                                               uint32_t tile, uint32_t ngroups, uint32_t unit, uint32_t gqa,
-                                               const int4_t *a, const float *step) {
+struct Tile {
+  static constexpr int kLoads = 2 * D / 64;
+  static constexpr int kStride = 2 * D + 16;  // of a record in LDS: the 16 lanes of a read lie in different banks
+  int4_t b[kLoads];
+  float scale;  // of group n
+  __device__ __forceinline__ void load(const int8_t *__restrict__ codes, const float *__restrict__ scales, uint32_t tile,
+                                       uint32_t ngroups) {
+    constexpr int kL = 2 * D / 16;  // lanes of a record
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const size_t g = min(16 * tile + j * (64 / kL) + lane / kL, ngroups - 1);
+      b[j] = *reinterpret_cast<const int4_t *>(codes + g * (2 * D) + 16 * (lane % kL));
+    }
+    scale = scales[min(16 * tile + (lane & 15), ngroups - 1)];
+  }
+  // Lane (kb, n) gets the products of group n with the heads 4 kb .. 4 kb + 3; lds: the wavefront's, 16 records.
+  __device__ __forceinline__ int4_t products(const int4_t *a, int8_t *lds) const {
+    constexpr int kL = 2 * D / 16;
+    const int lane = threadIdx.x & 63, n = lane & 15, kb = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      *reinterpret_cast<int4_t *>(lds + (j * (64 / kL) + lane / kL) * kStride + 16 * (lane % kL)) = b[j];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    int4_t c = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < kLoads; ++s)
+      c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], *reinterpret_cast<const int4_t *>(lds + n * kStride + 64 * s + 16 * kb), c,
+                                                0, 0, 0);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    return c;
+  }
+};
+
+// Keys (sortable scores) of a tile's units: lane n of the first sixteen has its group's (unit 1) or its pair's (unit 2) key,
+// 0 where nothing is visible.
+__device__ __forceinline__ uint32_t tile_keys(int4_t c, float scale, uint32_t tile, uint32_t ngroups, uint32_t unit, uint32_t gqa,
+                                              const float *step) {
   const int lane = threadIdx.x & 63, n = lane & 15, kb = lane >> 4;
-  const uint32_t g = 16 * tile + n;
-  const size_t gc = min(g, ngroups - 1);
-  const int8_t *rec = codes + gc * (2 * D) + 16 * kb;
-  constexpr int kSteps = 2 * D / 64;
-  int4_t b[kSteps];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) b[s] = *reinterpret_cast<const int4_t *>(rec + 64 * s);
-  const float scale = scales[gc];
-  int4_t c = {0, 0, 0, 0};
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b[s], c, 0, 0, 0);
-  float best = -INFINITY;  // rows 4 kb .. 4 kb + 3; a head whose step is not finite gives a NaN, which fmaxf passes over
+  float best = -INFINITY;  // a head whose step is not finite gives a NaN, which fmaxf passes over
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (static_cast<uint32_t>(4 * kb + r) < gqa) best = fmaxf(best, static_cast<float>(c[r]) * step[r]);
   best = cfd::rows4_max(best);
-  uint32_t key = g < ngroups ? cfsel::sortable(best * scale) : 0u;
+  uint32_t key = 16 * tile + n < ngroups ? cfsel::sortable(best * scale) : 0u;
   if (unit == 2) key = max(key, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(key), 0xb1, 0xf, 0xf, false)));
   return key;
 }
@@ -174,36 +212,44 @@ struct QueryOperand {
   }
 };
 
-constexpr int kScoreThreads = 256;
-
-// Scores to the workspace: grid (workgroups of a row, KV heads, sequences).
-template <int D>
-__global__ __launch_bounds__(kScoreThreads) void score_kernel(cf_kv_select_desc d, uint32_t *__restrict__ keys,
-                                                              uint32_t row_units) {
-  __shared__ __attribute__((aligned(16))) int8_t s_a[kRows][2 * D];
-  __shared__ float s_step[kRows];
-  const uint32_t head = blockIdx.y, seq = blockIdx.z, unit = d.unit_groups;
-  const uint32_t ngroups = (visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups) + 63) / 64;
-  const uint32_t tiles = (ngroups + 15) / 16, per = kScoreThreads / 64;
-  if (blockIdx.x * per >= tiles) return;
-  stage_query<D>(d, seq, head, s_a, s_step, kScoreThreads);
-  __syncthreads();
-  QueryOperand<D> q;
-  q.load(s_a, s_step);
+// Scores of the tiles wave0, wave0 + nwaves, ... of a row; put(unit, key) receives them. Two tiles at a time, the next
+// ones' records loaded into their registers as soon as the products are formed (8 KiB a wavefront in flight at D = 128); the
+// first ones' before the queries are staged. All threads of the workgroup call this.
+template <int D, typename Put>
+__device__ __forceinline__ void score_row(const cf_kv_select_desc &d, uint32_t seq, uint32_t head, uint32_t ngroups, uint32_t wave0,
+                                          uint32_t nwaves, int nthreads, int8_t (*s_a)[2 * D], float *s_step,
+                                          int8_t (*s_rec)[16 * Tile<D>::kStride], const Put &put) {
   const size_t row = static_cast<size_t>(seq) * d.kv_head_count + head;
   const int8_t *codes = d.codes + row * d.max_groups * (2 * D);
   const float *scales = d.scales + row * d.max_groups;
+  const uint32_t tiles = (ngroups + 15) / 16, unit = d.unit_groups, gqa = d.query_head_count / d.kv_head_count;
   const int lane = threadIdx.x & 63;
-  for (uint32_t t = blockIdx.x * per + (threadIdx.x >> 6); t < tiles; t += gridDim.x * per) {
-    const uint32_t key = score_tile<D>(codes, scales, t, ngroups, unit, d.query_head_count / d.kv_head_count, q.a, q.step);
-    if (lane < 16 && lane % unit == 0) {
-      const uint32_t u = (16 * t + lane) / unit;
-      if (u < row_units) keys[row * row_units + u] = key;
+  Tile<D> t[2];
+#pragma unroll
+  for (uint32_t j = 0; j < 2; ++j)
+    if (wave0 + j * nwaves < tiles) t[j].load(codes, scales, wave0 + j * nwaves, ngroups);
+  stage_query<D>(d, seq, head, s_a, s_step, nthreads);
+  __syncthreads();
+  QueryOperand<D> q;
+  q.load(s_a, s_step);
+  for (uint32_t i = wave0; i < tiles; i += 2 * nwaves) {
+    int4_t c[2];
+    float scale[2];
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      c[j] = t[j].products(q.a, s_rec[threadIdx.x >> 6]);
+      scale[j] = t[j].scale;
+      if (i + (j + 2) * nwaves < tiles) t[j].load(codes, scales, i + (j + 2) * nwaves, ngroups);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint32_t tile = i + j * nwaves;
+      if (tile >= tiles) break;
+      const uint32_t key = tile_keys(c[j], scale[j], tile, ngroups, unit, gqa, q.step);
+      if (lane < 16 && lane % unit == 0) put((16 * tile + lane) / unit, key);
     }
   }
 }
-
-constexpr int kPickThreads = 512;
 
 __device__ __forceinline__ void fill_none(uint32_t *p, uint32_t from, uint32_t to, int nthreads) {
   for (uint32_t i = from + threadIdx.x; i < to; i += nthreads) p[i] = CF_KV_NO_UNIT;
@@ -222,19 +268,88 @@ __device__ __forceinline__ void pick_units(const cf_kv_select_desc &d, size_t ro
   fill_none(out, k, d.max_units, T);
 }
 
-// The best units of each row from the scores in the workspace: grid (KV heads, sequences).
+__device__ __forceinline__ uint32_t visible_units(const cf_kv_select_desc &d, uint32_t ngroups) {
+  return (ngroups + d.unit_groups - 1) / d.unit_groups;
+}
+
+// A row's scores and its best units in one workgroup of T threads, the keys in LDS: grid (KV heads, sequences).
+constexpr uint32_t row_units_most(int T) { return T == 1024 ? 8192 : 2048; }
+
+template <int D, int T>
+__global__ __launch_bounds__(T) void select_row_kernel(cf_kv_select_desc d) {
+  __shared__ __attribute__((aligned(16))) int8_t s_a[kRows][2 * D];
+  __shared__ float s_step[kRows];
+  __shared__ uint32_t s_key[row_units_most(T)];
+  __shared__ __attribute__((aligned(16))) int8_t s_rec[T / 64][16 * Tile<D>::kStride];
+  __shared__ cfsel::TopkShared<T> sh;
+  const uint32_t head = blockIdx.x, seq = blockIdx.y;
+  const uint32_t ngroups = (visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups) + 63) / 64;
+  const uint32_t n = visible_units(d, ngroups);
+  if (n > d.max_units) {
+    score_row<D>(d, seq, head, ngroups, threadIdx.x >> 6, T / 64, T, s_a, s_step, s_rec, [&](uint32_t u, uint32_t key) {
+      if (u < n) s_key[u] = key;
+    });
+    __syncthreads();
+  }
+  pick_units<T>(d, static_cast<size_t>(seq) * d.kv_head_count + head, n, s_key, sh);
+}
+
+template <int D>
+void launch_rows(const cf_kv_select_desc &d, int threads, hipStream_t s) {
+  const dim3 grid(d.kv_head_count, d.seq_count);
+  if (threads == 1024) select_row_kernel<D, 1024><<<grid, 1024, 0, s>>>(d);
+  else select_row_kernel<D, 256><<<grid, 256, 0, s>>>(d);
+}
+
+// Two launches: scores to the workspace, grid (workgroups of a row, KV heads, sequences) ...
+constexpr int kScoreThreads = 256;
+
+template <int D>
+__global__ __launch_bounds__(kScoreThreads) void score_kernel(cf_kv_select_desc d, uint32_t *__restrict__ keys,
+                                                              uint32_t row_units) {
+  __shared__ __attribute__((aligned(16))) int8_t s_a[kRows][2 * D];
+  __shared__ float s_step[kRows];
+  __shared__ __attribute__((aligned(16))) int8_t s_rec[kScoreThreads / 64][16 * Tile<D>::kStride];
+  const uint32_t head = blockIdx.y, seq = blockIdx.z;
+  const uint32_t ngroups = (visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups) + 63) / 64;
+  constexpr uint32_t kPer = kScoreThreads / 64;
+  if (16 * blockIdx.x * kPer >= ngroups) return;
+  uint32_t *out = keys + (static_cast<size_t>(seq) * d.kv_head_count + head) * row_units;
+  score_row<D>(d, seq, head, ngroups, blockIdx.x * kPer + (threadIdx.x >> 6), gridDim.x * kPer, kScoreThreads, s_a, s_step, s_rec,
+               [&](uint32_t u, uint32_t key) {
+                 if (u < row_units) out[u] = key;
+               });
+}
+
+// ... and the best units of each row from there: grid (KV heads, sequences).
+constexpr int kPickThreads = 1024;
+
 __global__ __launch_bounds__(kPickThreads) void pick_kernel(cf_kv_select_desc d, const uint32_t *__restrict__ keys,
                                                             uint32_t row_units) {
   __shared__ cfsel::TopkShared<kPickThreads> sh;
   const uint32_t head = blockIdx.x, seq = blockIdx.y;
-  const uint32_t span = 64 * d.unit_groups;
-  const uint32_t vis = visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups);
-  const uint32_t n = vis / span + (vis % span != 0);
+  const uint32_t ngroups = (visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups) + 63) / 64;
   const size_t row = static_cast<size_t>(seq) * d.kv_head_count + head;
-  pick_units<kPickThreads>(d, row, n, keys + row * row_units, sh);
+  pick_units<kPickThreads>(d, row, visible_units(d, ngroups), keys + row * row_units, sh);
 }
 
 uint32_t row_units(const cf_kv_select_desc *d) { return (d->max_groups + d->unit_groups - 1) / d->unit_groups; }
+
+// Threads of the one workgroup that takes a row, 0 for two launches (scores of a row over many workgroups, then the pick).
+// us at 32 query / 8 KV heads, head_dim 128, as 256 threads / 1024 threads / two launches:
+//   rows x groups      8 x 128    8.2 /  8.7 / 11.2      8 x 1024  16.4 / 12.2 / 11.8      32 x 2048  25.7 / 16.7 / 15.9
+//                    256 x 512   12.0 / 11.2 / 15.9    128 x 2048  26.6 / 19.2 / 22.2     256 x 2048  30.7 / 27.8 / 32.5
+//                    512 x 128   10.2 / 16.5 / 18.3   1024 x 128   15.8 / 31.0 / 25.6    1024 x 512   26.6 / 47.7 / 40.4
+// Workgroups of 256 threads leave several a CU: for more rows than CUs, and for rows too short to keep more wavefronts busy.
+// One CU reads a row at some 70 GB/s, which loses to two launches when the row is long and other CUs would be idle.
+int row_threads(const cf_kv_select_desc *d) {
+  const uint32_t units = row_units(d);
+  const uint64_t rows = static_cast<uint64_t>(d->seq_count) * d->kv_head_count;
+  const uint64_t row_bytes = static_cast<uint64_t>(d->max_groups) * 2 * d->head_dim;
+  if (units <= row_units_most(256) && (rows > cfd::cu_count() || row_bytes <= (32u << 10))) return 256;
+  if (units <= row_units_most(1024) && (rows >= 64 || row_bytes <= (256u << 10))) return 1024;
+  return 0;
+}
 
 // ---- eviction ---------------------------------------------------------------------------------------------------
 constexpr int kEvictThreads = 256;
@@ -385,7 +500,7 @@ extern "C" cf_status cf_kv_validate_select_desc(const cf_kv_select_desc *d) {
 }
 
 extern "C" uint64_t cf_kv_select_workspace_bytes(const cf_kv_select_desc *d) {
-  if (cf_kv_validate_select_desc(d) != CF_OK) return 0;
+  if (cf_kv_validate_select_desc(d) != CF_OK || row_threads(d)) return 0;
   return static_cast<uint64_t>(d->seq_count) * d->kv_head_count * row_units(d) * sizeof(uint32_t);
 }
 
@@ -395,10 +510,19 @@ extern "C" cf_status cf_kv_select_groups_async(const cf_kv_select_desc *d, void 
   const uint64_t need = cf_kv_select_workspace_bytes(d);
   if (need && (!d->workspace || d->workspace_bytes < need || !aligned16(d->workspace))) return CF_ERR_INVALID_ARGUMENT;
   const hipStream_t s = cfd::as_stream(stream);
+  if (const int threads = row_threads(d)) {
+    if (d->head_dim == 128) launch_rows<128>(*d, threads, s);
+    else launch_rows<64>(*d, threads, s);
+    return cfd::launch_status();
+  }
   const uint32_t units = row_units(d);
   uint32_t *keys = static_cast<uint32_t *>(d->workspace);
   const uint32_t tiles = (d->max_groups + 15) / 16, per = kScoreThreads / 64;
-  const dim3 grid(std::min<uint32_t>((tiles + per - 1) / per, 1u << 16), d->kv_head_count, d->seq_count);
+  // wavefronts of about 4 tiles where there are enough rows to fill the chip with them
+  const uint64_t rows = static_cast<uint64_t>(d->kv_head_count) * d->seq_count;
+  const uint32_t most = std::max<uint32_t>((tiles + per - 1) / per, 1u);
+  const uint64_t want = std::max<uint64_t>((most + 3) / 4, (4ull * cfd::cu_count() + rows - 1) / rows);
+  const dim3 grid(static_cast<uint32_t>(std::min<uint64_t>({want, most, 1u << 16})), d->kv_head_count, d->seq_count);
   if (d->head_dim == 128) score_kernel<128><<<grid, kScoreThreads, 0, s>>>(*d, keys, units);
   else score_kernel<64><<<grid, kScoreThreads, 0, s>>>(*d, keys, units);
   pick_kernel<<<dim3(d->kv_head_count, d->seq_count), kPickThreads, 0, s>>>(*d, keys, units);

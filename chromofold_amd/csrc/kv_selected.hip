@@ -33,22 +33,25 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float4a4_t __attribute__((ext_vector_type(4), aligned(4)));  // queries need no more than a float's alignment
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kHdr = 64;
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kWaves = 4;     // of a workgroup that takes part of a row
+constexpr int kWavesRow = 8;  // of a workgroup that takes a whole row
 constexpr int kRows = 16;
 constexpr int kPStride = 80;  // halves of a row of the weight tile: the four rows a store instruction writes start 32 banks apart
+constexpr uint32_t kRowStats = 2048;  // group statistics that a workgroup with a whole row holds in LDS
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct SelArgs {
   cf_kv_batched_desc d;
   cf_kv_selection s;
-  uint32_t slots;    // list entries (groups) of a row: max_units * unit_groups, or max_groups without a list
+  uint32_t slots;    // the most slots of a row: max_units * unit_groups list entries, or max_groups without a list
   uint32_t splits;   // workgroups of a row
   uint32_t per;      // slots of a workgroup
-  float *states;     // [row][split][gqa][D + 2]: sum of p v, then maximum (log2 units) and sum of p
+  float *sums;       // [row][split][gqa][D]: sum of p v
+  float2 *states;    // [row][split][gqa]: maximum (log2 units) and sum of p
   float2 *stats;     // [row][slot][gqa]: a group's maximum (log2 units) and sum of exp2(score - maximum)
 };
 
@@ -83,69 +86,112 @@ __device__ __forceinline__ uint32_t listed_group(const SelArgs &a, const uint32_
   return x >= a.d.max_groups ? 0xFFFFFFFFu : x * a.s.unit_groups + j;
 }
 
-template <int D>
-__global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
+// Slots of a row: with a list, the entries that can name a visible unit.
+__device__ __forceinline__ uint32_t row_slots(const SelArgs &a, uint32_t ngroups) {
+  return a.s.units ? min(a.slots, (ngroups + a.s.unit_groups - 1) / a.s.unit_groups * a.s.unit_groups) : ngroups;
+}
+
+// Weight of a group from its heads' statistics, the row's maxima and the inverse sums.
+template <typename Stat>
+__device__ __forceinline__ float group_weight(const Stat &stat, uint32_t gqa, const float *m, const float *inv_l) {
+  float w = 0.0f;
+  for (uint32_t h0 = 0; h0 < gqa; h0 += 4) {
+    float2 x[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) x[j] = stat(min(h0 + j, gqa - 1));
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+      if (h0 + j < gqa && x[j].x != -INFINITY) w += x[j].y * __builtin_amdgcn_exp2f(x[j].x - m[h0 + j]) * inv_l[h0 + j];
+  }
+  return w;
+}
+
+// The row's weights of groups [lo, hi): decayed, then the listed ones' shares added. All threads of the workgroup call this.
+template <typename Stat>
+__device__ __forceinline__ void write_weights(const SelArgs &a, size_t row, const uint32_t *list, uint32_t ngroups, uint32_t nslots,
+                                              uint32_t lo, uint32_t hi, uint32_t gqa, const float *m, const float *inv_l, const Stat &stat) {
+  const float *in = a.s.weights_in ? a.s.weights_in + row * a.d.max_groups : nullptr;
+  float *out = a.s.weights_out + row * a.d.max_groups;
+  if (!list) {
+    for (uint32_t g = lo + threadIdx.x; g < hi; g += blockDim.x) {
+      const float w = in ? a.s.decay * in[g] : 0.0f;
+      out[g] = g < ngroups ? w + group_weight([&](uint32_t h) { return stat(g, h); }, gqa, m, inv_l) : w;
+    }
+    return;
+  }
+  for (uint32_t g = lo + threadIdx.x; g < hi; g += blockDim.x) out[g] = in ? a.s.decay * in[g] : 0.0f;
+  __syncthreads();
+  for (uint32_t s = threadIdx.x; s < nslots; s += blockDim.x) {
+    bool bad = false;
+    const uint32_t g = listed_group(a, list, s, bad);
+    if (g < ngroups && g >= lo && g < hi) out[g] += group_weight([&](uint32_t h) { return stat(s, h); }, gqa, m, inv_l);
+  }
+}
+
+// ROW: the workgroup has the row to itself and finishes it; its groups' statistics stay in LDS.
+template <int D, int W, bool ROW>
+__global__ __launch_bounds__(64 * W, 2) void selected_kernel(SelArgs a) {
   constexpr int kSteps = D / 32;   // k-steps of q . k
   constexpr int kTiles = D / 16;   // dim tiles of p . v
   constexpr int kKLoads = D / 16;  // 16-byte loads of a lane: K
   constexpr int kVLoads = D / 4;   // 4-byte loads of a lane: V
-  constexpr int kState = kRows * (D + 2);
   __shared__ union {
-    struct {
-      _Float16 p[kWaves][2][kRows][kPStride];
-    };
-    float red[kWaves][kState];
-    _Float16 q[2][kRows][D];
+    _Float16 p[W][2][kRows][kPStride];
+    float red[W][kRows][D];
   } sh;
-  __shared__ float s_unit[kRows];  // log2-unit factor of a row's scores, without the page's scale
-  __shared__ float s_m[kWaves][kRows];
+  __shared__ float s_m[W][kRows], s_l[W][kRows];
+  __shared__ float s_top[kRows], s_inv[kRows];
+  __shared__ float2 s_stat[ROW ? kRowStats : 1];
 
   const int lane = threadIdx.x & 63, n = lane & 15, b = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t split = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
   const uint32_t gqa = a.d.query_head_count / a.d.kv_head_count;
   const size_t row = static_cast<size_t>(seq) * a.d.kv_head_count + head;
-  const uint32_t visible = visible_tokens(a.d.seq_tokens[seq], a.d.query_pos[seq], a.d.max_groups);
-  const uint32_t ngroups = (visible + 63) / 64;
-  const uint32_t s0 = min(split * a.per, a.slots);
   const uint32_t *list = a.s.units ? a.s.units + row * a.s.max_units : nullptr;
-  const uint32_t s1 = min(list ? a.slots : ngroups, s0 + a.per);
   const uint32_t *grow = a.d.group_offsets + row * a.d.max_groups;
+  auto put_stat = [&](uint32_t slot, uint32_t h, float m, float l) {
+    if constexpr (ROW) s_stat[slot * gqa + h] = float2{m, l};
+    else a.stats[(row * a.slots + slot) * gqa + h] = float2{m, l};
+  };
 
-  // ---- queries: each head's in units of a power of two that puts its largest element into [2^14, 2^15)
-  for (int h = wave; h < kRows; h += kWaves) {
-    constexpr int kN = D / 64;
-    const float *q = a.d.queries + (static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + h) * D;
-    float x[kN], top = 0.0f;
+  // ---- queries, straight from memory into the layout of the A operands: row n, dims 4 (8 s + b) .. + 3 and
+  // 4 (8 s + 4 + b) .. + 3 of step s. Their loads come first, so that they are there when the list entry and the offset,
+  // which the first group waits for anyway, have come.
+  const float *qrow = a.d.queries + (static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + min(static_cast<uint32_t>(n), gqa - 1)) * D;
+  float4_t qx[2 * kSteps];
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      x[j] = static_cast<uint32_t>(h) < gqa ? q[lane + 64 * j] : 0.0f;
-      top = fmaxf(top, fabsf(x[j]));
-    }
+  for (int s = 0; s < 2 * kSteps; ++s) qx[s] = *reinterpret_cast<const float4a4_t *>(qrow + 4 * (4 * s + b));
+
+  const uint32_t visible = visible_tokens(a.d.seq_tokens[seq], a.d.query_pos[seq], a.d.max_groups);
+  const uint32_t ngroups = (visible + 63) / 64, nslots = row_slots(a, ngroups);
+  const uint32_t s0 = ROW ? 0 : min(split * a.per, nslots), s1 = ROW ? nslots : min(nslots, s0 + a.per);
+
+  half8_t qh[kSteps], ql[kSteps];
+  float unit[4];  // log2-unit factor of the rows' scores, without the page's scale
+  // each head in units of a power of two that puts its largest element into [2^14, 2^15)
+  auto split_queries = [&] {
+    float top = 0.0f;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    for (int s = 0; s < 2 * kSteps; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(qx[s][j]));
+    top = cfd::rows4_max(top);
     const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+    const float u = ldexpf(a.d.softmax_scale * kLog2e, e);
 #pragma unroll
-    for (int j = 0; j < kN; ++j)
-      cfd::split_mul_f16(ldexpf(x[j], -e), 1.0f, sh.q[0][h][lane + 64 * j], sh.q[1][h][lane + 64 * j]);
-    if (lane == 0) s_unit[h] = ldexpf(a.d.softmax_scale * kLog2e, e);
-  }
-  __syncthreads();
-  half8_t qh[kSteps], ql[kSteps];  // A operands: row n, dims 4 (8 s + b) .. + 3 and 4 (8 s + 4 + b) .. + 3
+    for (int r = 0; r < 4; ++r) unit[r] = __shfl(u, 4 * b + r);
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    auto get = [&](int part) {
-      const half4_t x = *reinterpret_cast<const half4_t *>(&sh.q[part][n][4 * (8 * s + b)]);
-      const half4_t y = *reinterpret_cast<const half4_t *>(&sh.q[part][n][4 * (8 * s + 4 + b)]);
-      return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    qh[s] = get(0);
-    ql[s] = get(1);
-  }
-  float unit[4];
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-  for (int r = 0; r < 4; ++r) unit[r] = s_unit[4 * b + r];
-  __syncthreads();  // the query area becomes the weight tiles
+      for (int j = 0; j < 8; ++j) {
+        const float x = static_cast<uint32_t>(n) < gqa ? ldexpf(qx[2 * s + j / 4][j % 4], -e) : 0.0f;
+        _Float16 hi, lo;
+        cfd::split_mul_f16(x, 1.0f, hi, lo);
+        qh[s][j] = hi;
+        ql[s][j] = lo;
+      }
+  };
 
   float m_run[4], l_run[4];
 #pragma unroll
@@ -154,12 +200,12 @@ __global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
   float4_t acc[kTiles];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) acc[i] = float4_t{0, 0, 0, 0};
-  bool bad = false;
+  bool bad = false, split_done = false;
 
-  // The wavefront's slots s0 + wave, + kWaves, ...: 64 of them at a time, one a lane, so that no load of the loop below
+  // The wavefront's slots s0 + wave, + W, ...: 64 of them at a time, one a lane, so that no load of the loop below
   // waits for a list entry or an offset.
-  for (uint32_t c0 = s0 + wave; c0 < s1; c0 += 64 * kWaves) {
-    const uint32_t mine = c0 + lane * kWaves;
+  for (uint32_t c0 = s0 + wave; c0 < s1; c0 += 64 * W) {
+    const uint32_t mine = c0 + lane * W;
     uint32_t g_l = 0xFFFFFFFFu, off_l = 0;
     if (mine < s1) {
       g_l = listed_group(a, list, mine, bad);
@@ -168,7 +214,7 @@ __global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
     const bool here = g_l < ngroups;
     uint64_t todo = __builtin_amdgcn_ballot_w64(here);
     if (a.s.weights_out && mine < s1 && !here)
-      for (uint32_t h = 0; h < gqa; ++h) a.stats[(row * a.slots + mine) * gqa + h] = float2{-INFINITY, 0.0f};
+      for (uint32_t h = 0; h < gqa; ++h) put_stat(mine, h, -INFINITY, 0.0f);
     if (!todo) continue;
 
     uint4_t kw[kKLoads];
@@ -198,6 +244,8 @@ __global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
     const uint8_t *blob = blob_of(cur);
     load_k(blob);
     load_v(blob);
+    if (!split_done) split_queries();
+    split_done = true;
     for (;;) {
       const int next = todo ? __builtin_ctzll(todo) : -1;
       todo &= todo - 1;
@@ -208,13 +256,15 @@ __global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) sc[i] = float4_t{0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kSteps; ++s) {
+        half8_t k[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const half8_t k = signed_half8(kw[2 * s][i], kw[2 * s + 1][i]);
-          sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[s], k, sc[i], 0, 0, 0);
-          sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[s], k, sc[i], 0, 0, 0);
-        }
+        for (int i = 0; i < 4; ++i) k[i] = signed_half8(kw[2 * s][i], kw[2 * s + 1][i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[s], k[i], sc[i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[s], k[i], sc[i], 0, 0, 0);
+      }
       bad |= codec != CF_KV_CODEC_INT8 || dim != D;
       // tokens of a page are visible from its first on
       const uint32_t page_end = 64 * g + 16 * (n >> 2) + min(tc, 16u);
@@ -270,24 +320,21 @@ __global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
         l_run[r] += sum[r];
       }
       if (a.s.weights_out) {
-        const size_t at = (row * a.slots + c0 + static_cast<uint32_t>(cur) * kWaves) * gqa;
+        const uint32_t slot = c0 + static_cast<uint32_t>(cur) * W;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float t = cfd::row16_sum(sum[r]);
-          if (n == r && static_cast<uint32_t>(4 * b + r) < gqa) a.stats[at + 4 * b + r] = float2{m_run[r], t};
+          if (n == r && static_cast<uint32_t>(4 * b + r) < gqa) put_stat(slot, 4 * b + r, m_run[r], t);
         }
       }
       if (static_cast<uint32_t>(4 * b) < gqa) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          half4_t hi, lo;
           _Float16 h0, l0, h1, l1, h2, l2, h3, l3;
           cfd::split2_mul_f16(p[0][r], p[1][r], vsn, h0, l0, h1, l1);
           cfd::split2_mul_f16(p[2][r], p[3][r], vsn, h2, l2, h3, l3);
-          hi = half4_t{h0, h1, h2, h3};
-          lo = half4_t{l0, l1, l2, l3};
-          *reinterpret_cast<half4_t *>(&sh.p[wave][0][4 * b + r][4 * n]) = hi;
-          *reinterpret_cast<half4_t *>(&sh.p[wave][1][4 * b + r][4 * n]) = lo;
+          *reinterpret_cast<half4_t *>(&sh.p[wave][0][4 * b + r][4 * n]) = half4_t{h0, h1, h2, h3};
+          *reinterpret_cast<half4_t *>(&sh.p[wave][1][4 * b + r][4 * n]) = half4_t{l0, l1, l2, l3};
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -299,10 +346,14 @@ __global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
         const half8_t ph = *reinterpret_cast<const half8_t *>(&sh.p[wave][0][n][16 * b + 8 * tp]);
         const half8_t pl = *reinterpret_cast<const half8_t *>(&sh.p[wave][1][n][16 * b + 8 * tp]);
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          const half8_t v = signed_half8(vw[2 * tp * kTiles + i], vw[(2 * tp + 1) * kTiles + i]);
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, v, acc[i], 0, 0, 0);
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, v, acc[i], 0, 0, 0);
+        for (int i0 = 0; i0 < kTiles; i0 += 4) {
+          half8_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = signed_half8(vw[2 * tp * kTiles + i0 + i], vw[(2 * tp + 1) * kTiles + i0 + i]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, v[i], acc[i0 + i], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, v[i], acc[i0 + i], 0, 0, 0);
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -321,144 +372,195 @@ __global__ __launch_bounds__(kThreads, 2) void selected_kernel(SelArgs a) {
   const bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
   if (n == 0) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)  // a NaN score leaves the maximum as it was and makes the sum a NaN
+    for (int r = 0; r < 4; ++r) {  // a NaN score leaves the maximum as it was and makes the sum a NaN
       s_m[wave][4 * b + r] = broken || l_run[r] != l_run[r] ? __builtin_nanf("") : m_run[r];
+      s_l[wave][4 * b + r] = l_run[r];
+    }
   }
   __syncthreads();  // (and the weight tiles are dead)
   if (static_cast<uint32_t>(4 * b) < gqa) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float *o = sh.red[wave] + (4 * b + r) * (D + 2);
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) o[16 * i + n] = ldexpf(acc[i][r], max(e_run, -200));
-      if (n == 0) o[D] = l_run[r];
-    }
+      for (int i = 0; i < kTiles; ++i) sh.red[wave][4 * b + r][16 * i + n] = ldexpf(acc[i][r], max(e_run, -200));
   }
   __syncthreads();
-  float *st = a.states + (row * a.splits + split) * gqa * (D + 2);
-  for (uint32_t i = threadIdx.x; i < gqa * D; i += kThreads) {
+  const size_t at = (row * a.splits + split) * gqa;
+  for (uint32_t i = threadIdx.x; i < gqa * D; i += 64 * W) {
     const uint32_t h = i / D, dd = i % D;
     float m = -INFINITY, l = 0.0f, o = 0.0f;
     bool nan = false;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       nan |= s_m[w][h] != s_m[w][h];
       m = fmaxf(m, s_m[w][h]);
     }
     if (m != -INFINITY)
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < W; ++w) {
         if (s_m[w][h] == -INFINITY) continue;
         const float f = __builtin_amdgcn_exp2f(s_m[w][h] - m);
-        l += sh.red[w][h * (D + 2) + D] * f;
-        o += sh.red[w][h * (D + 2) + dd] * f;
+        l += s_l[w][h] * f;
+        o += sh.red[w][h][dd] * f;
       }
     if (nan) m = __builtin_nanf("");
-    if (a.splits == 1 && !a.s.weights_out) {
+    if constexpr (ROW) {
       a.d.output[(static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + h) * D + dd] =
           nan ? m : m == -INFINITY ? 0.0f : o / l;
-    } else {
-      st[h * (D + 2) + dd] = o;
       if (dd == 0) {
-        st[h * (D + 2) + D] = m;
-        st[h * (D + 2) + D + 1] = l;
+        s_top[h] = m;
+        s_inv[h] = 1.0f / l;
       }
+    } else {
+      a.sums[at * D + i] = o;
+      if (dd == 0) a.states[at + h] = float2{m, l};
     }
+  }
+  if constexpr (ROW) {
+    if (!a.s.weights_out) return;
+    __syncthreads();
+    write_weights(a, row, list, ngroups, nslots, 0, a.d.max_groups, gqa, s_top, s_inv,
+                  [&](uint32_t slot, uint32_t h) { return s_stat[slot * gqa + h]; });
   }
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
+constexpr uint32_t kJoinGroups = 1024;  // groups whose weights one workgroup writes
 
-// Joins a row's workgroups and turns group statistics into weights: grid (KV heads, sequences).
+// Joins a row's states: grid (KV heads, sequences, query heads + parts of the weights). A workgroup z < gqa makes the
+// output of query head z; the others turn group statistics into weights, kJoinGroups groups each. Values of many states are
+// loaded at a time: the caches of other dies hold them, so that each load takes about a microsecond.
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a) {
-  __shared__ float s_m[kRows], s_l[kRows];
-  const uint32_t head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+  constexpr int kParts = kJoinThreads / D;
+  constexpr uint32_t kB = 8;
+  __shared__ float s_m[kRows], s_inv[kRows];
+  __shared__ float s_o[kParts][D];
+  const uint32_t head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const uint32_t gqa = a.d.query_head_count / a.d.kv_head_count;
   const size_t row = static_cast<size_t>(seq) * a.d.kv_head_count + head;
-  const float *st = a.states + row * a.splits * gqa * (D + 2);
-  const size_t stride = static_cast<size_t>(gqa) * (D + 2);
-  for (uint32_t i = tid; i < gqa * D; i += kJoinThreads) {
-    const uint32_t h = i / D, dd = i % D;
-    const float *p = st + h * (D + 2);
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
+  const size_t state0 = row * a.splits;
+  const uint32_t states = a.splits;
+  const float2 *st = a.states + state0 * gqa;
+  const bool out = blockIdx.z < gqa;
+  // the sums of this thread's first states, in flight while the maxima are found
+  const uint32_t part = tid / D, dd = tid % D;
+  const float *sums = a.sums + (state0 * gqa + (out ? blockIdx.z : 0)) * D + dd;
+  float o8[kB];
+#pragma unroll
+  for (uint32_t u = 0; u < kB; ++u)
+    o8[u] = out ? sums[static_cast<size_t>(min(part + u * kParts, states - 1)) * gqa * D] : 0.0f;
+  // a wavefront per query head: its maximum and the inverse of its sum
+  for (uint32_t h = out ? blockIdx.z : tid >> 6; h < (out ? blockIdx.z + 1 : gqa); h += kJoinThreads / 64) {
+    float m = -INFINITY, l = 0.0f;
     bool nan = false;
-    for (uint32_t s = 0; s < a.splits; ++s) {
-      const float x = p[s * stride + D];
-      nan |= x != x;
-      m = fmaxf(m, x);
-    }
-    if (m != -INFINITY)
-      for (uint32_t s = 0; s < a.splits; ++s) {
-        const float x = p[s * stride + D];
-        if (x == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(x - m);
-        l += p[s * stride + D + 1] * f;
-        o += p[s * stride + dd] * f;
+    for (uint32_t s = lane; s < states; s += 64) {
+      const float2 x = st[static_cast<size_t>(s) * gqa + h];
+      nan |= x.x != x.x;
+      const float mn = fmaxf(m, x.x);
+      if (mn != -INFINITY) {
+        l = (m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - mn)) +
+            (x.x == -INFINITY ? 0.0f : x.y * __builtin_amdgcn_exp2f(x.x - mn));
+        m = mn;
       }
-    if (nan) m = __builtin_nanf("");
-    a.d.output[(static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + h) * D + dd] =
-        nan ? m : m == -INFINITY ? 0.0f : o / l;
-    if (dd == 0) {
-      s_m[h] = m;
-      s_l[h] = l;
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
+    l = m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) l += __shfl_xor(l, k);
+    nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    if (lane == 0) {
+      s_m[h] = nan ? __builtin_nanf("") : top;
+      s_inv[h] = 1.0f / l;
     }
   }
-  if (!a.s.weights_out) return;
-  const uint32_t visible = visible_tokens(a.d.seq_tokens[seq], a.d.query_pos[seq], a.d.max_groups);
-  const uint32_t ngroups = (visible + 63) / 64;
-  const float *in = a.s.weights_in ? a.s.weights_in + row * a.d.max_groups : nullptr;
-  float *out = a.s.weights_out + row * a.d.max_groups;
-  const uint32_t *list = a.s.units ? a.s.units + row * a.s.max_units : nullptr;
-  for (uint32_t g = tid; g < a.d.max_groups; g += kJoinThreads) out[g] = in ? a.s.decay * in[g] : 0.0f;
-  __syncthreads();  // s_m, s_l; the decayed weights of the whole row
-  for (uint32_t s = tid; s < (list ? a.slots : ngroups); s += kJoinThreads) {
-    bool bad = false;
-    const uint32_t g = listed_group(a, list, s, bad);
-    if (g >= ngroups) continue;
-    float w = 0.0f;
-    for (uint32_t h = 0; h < gqa; ++h) {
-      const float2 x = a.stats[(row * a.slots + s) * gqa + h];
-      if (x.x != -INFINITY) w += x.y * __builtin_amdgcn_exp2f(x.x - s_m[h]) / s_l[h];
+  __syncthreads();
+  if (out) {
+    const float m = s_m[blockIdx.z];
+    float o = 0.0f;
+    if (m != -INFINITY)
+      for (uint32_t s = part; s < states; s += kB * kParts) {
+        float x[kB], f[kB];
+#pragma unroll
+        for (uint32_t u = 0; u < kB; ++u) {
+          const size_t i = static_cast<size_t>(min(s + u * kParts, states - 1)) * gqa;
+          f[u] = st[i + blockIdx.z].x;
+          x[u] = s == part ? o8[u] : sums[i * D];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kB; ++u)
+          if (s + u * kParts < states && f[u] != -INFINITY) o += x[u] * __builtin_amdgcn_exp2f(f[u] - m);
+      }
+    s_o[part][dd] = o;
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int k = 1; k < kParts; ++k) o += s_o[k][dd];
+      a.d.output[(static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + blockIdx.z) * D + dd] =
+          m != m ? m : m == -INFINITY ? 0.0f : o * s_inv[blockIdx.z];
     }
-    out[g] += w;
+    return;
   }
+  const uint32_t ngroups = (visible_tokens(a.d.seq_tokens[seq], a.d.query_pos[seq], a.d.max_groups) + 63) / 64;
+  const uint32_t lo = (blockIdx.z - gqa) * kJoinGroups, hi = min(lo + kJoinGroups, a.d.max_groups);
+  const float2 *stats = a.stats + row * a.slots * gqa;
+  write_weights(a, row, a.s.units ? a.s.units + row * a.s.max_units : nullptr, ngroups, row_slots(a, ngroups), lo, hi, gqa, s_m,
+                s_inv, [&](uint32_t slot, uint32_t h) { return stats[static_cast<size_t>(slot) * gqa + h]; });
 }
 
 struct Plan {
+  bool row;
   uint32_t slots, splits, per;
-  uint64_t state_bytes, stat_bytes;
+  uint64_t sum_bytes, state_bytes, stat_bytes;
+  uint64_t bytes() const { return sum_bytes + state_bytes + stat_bytes; }
 };
+
+uint64_t round16(uint64_t x) { return (x + 15) / 16 * 16; }
 
 Plan make_plan(const cf_kv_batched_desc *d, const cf_kv_selection *s) {
   Plan p{};
-  p.slots = d->max_groups;
-  if (s->units) p.slots = s->max_units * s->unit_groups;
-  const uint64_t rows = static_cast<uint64_t>(d->seq_count) * d->kv_head_count;
+  p.slots = s->units ? s->max_units * s->unit_groups : d->max_groups;
+  const uint64_t rows = static_cast<uint64_t>(d->seq_count) * d->kv_head_count, all = rows * p.slots;
+  const uint32_t gqa = d->query_head_count / d->kv_head_count, cus = cfd::cu_count();
+  const bool fits = static_cast<uint64_t>(p.slots) * gqa <= kRowStats;  // a row's statistics in LDS
   uint32_t splits = d->splits;
+  // One workgroup per row where its statistics fit and the rows fill the chip: a list makes them alike in length, and where
+  // there are many of them they even out. 248 rows of 64 listed groups: 47 us, against 53 to 61 as 2 to 8 splits and the
+  // second launch. Rows of unlike length that are not many (no list) would wait for the longest: those are split, which
+  // costs 256 rows of 512 groups each 349 us instead of 321.
+  if (splits == 0 && fits && ((s->units && 4 * rows >= 3 * cus) || rows >= 8 * cus)) splits = 1;
   if (splits == 0) {
     // one resident round of wavefronts (two workgroups of four per CU) where there are few slots, at most 16 slots a
     // wavefront where there are many
-    const uint64_t per_wave = std::min<uint64_t>(16, std::max<uint64_t>(1, rows * p.slots / (8ull * cfd::cu_count())));
+    const uint64_t per_wave = std::min<uint64_t>(16, std::max<uint64_t>(1, all / (8ull * cus)));
     splits = static_cast<uint32_t>((p.slots + per_wave * kWaves - 1) / (per_wave * kWaves));
   }
   splits = std::max<uint32_t>(1, std::min(splits, p.slots));
   p.per = (p.slots + splits - 1) / splits;
   p.splits = (p.slots + p.per - 1) / p.per;
-  const uint32_t gqa = d->query_head_count / d->kv_head_count;
-  const bool states = p.splits > 1 || s->weights_out;
-  p.state_bytes = states ? (rows * p.splits * gqa * (d->head_dim + 2) * sizeof(float) + 15) / 16 * 16 : 0;
-  p.stat_bytes = s->weights_out ? rows * p.slots * gqa * sizeof(float2) : 0;
+  p.row = p.splits == 1 && fits;
+  if (!p.row) {
+    p.sum_bytes = round16(rows * p.splits * gqa * d->head_dim * sizeof(float));
+    p.state_bytes = round16(rows * p.splits * gqa * sizeof(float2));
+    p.stat_bytes = s->weights_out ? all * gqa * sizeof(float2) : 0;
+  }
   return p;
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <int D>
-void launch(const SelArgs &a, hipStream_t s) {
-  selected_kernel<D><<<dim3(a.splits, a.d.kv_head_count, a.d.seq_count), kThreads, 0, s>>>(a);
-  if (a.splits > 1 || a.s.weights_out)
-    join_kernel<D><<<dim3(a.d.kv_head_count, a.d.seq_count), kJoinThreads, 0, s>>>(a);
+void launch(const SelArgs &a, bool row, hipStream_t s) {
+  const uint32_t heads = a.d.kv_head_count, seqs = a.d.seq_count;
+  if (row) {
+    selected_kernel<D, kWavesRow, true><<<dim3(1, heads, seqs), 64 * kWavesRow, 0, s>>>(a);
+    return;
+  }
+  selected_kernel<D, kWaves, false><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
+  const uint32_t parts = a.s.weights_out ? (a.d.max_groups + kJoinGroups - 1) / kJoinGroups : 0;
+  join_kernel<D><<<dim3(heads, seqs, a.d.query_head_count / heads + parts), kJoinThreads, 0, s>>>(a);
 }
 
 }  // namespace
@@ -490,21 +592,21 @@ extern "C" cf_status cf_kv_validate_selection(const cf_kv_batched_desc *d, const
 
 extern "C" uint64_t cf_kv_selected_workspace_bytes(const cf_kv_batched_desc *d, const cf_kv_selection *s) {
   if (cf_kv_validate_selection(d, s) != CF_OK) return 0;
-  const Plan p = make_plan(d, s);
-  return p.state_bytes + p.stat_bytes;
+  return make_plan(d, s).bytes();
 }
 
 extern "C" cf_status cf_kv_paged_attention_selected_async(const cf_kv_batched_desc *d, const cf_kv_selection *s, void *stream) {
   const cf_status v = cf_kv_validate_selection(d, s);
   if (v != CF_OK) return v;
   const Plan p = make_plan(d, s);
-  const uint64_t need = p.state_bytes + p.stat_bytes;
+  const uint64_t need = p.bytes();
   if (need && (!d->workspace || d->workspace_bytes < need || !aligned16(d->workspace))) return CF_ERR_INVALID_ARGUMENT;
-  SelArgs a{*d, *s, p.slots, p.splits, p.per, static_cast<float *>(d->workspace),
-            reinterpret_cast<float2 *>(static_cast<char *>(d->workspace) + p.state_bytes)};
+  char *ws = static_cast<char *>(d->workspace);
+  SelArgs a{*d, *s, p.slots, p.splits, p.per, reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.sum_bytes),
+            reinterpret_cast<float2 *>(ws + p.sum_bytes + p.state_bytes)};
   if (!s->units) a.s.unit_groups = 1;
   const hipStream_t st = cfd::as_stream(stream);
-  if (d->head_dim == 128) launch<128>(a, st);
-  else launch<64>(a, st);
+  if (d->head_dim == 128) launch<128>(a, p.row, st);
+  else launch<64>(a, p.row, st);
   return cfd::launch_status();
 }

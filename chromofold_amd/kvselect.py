@@ -53,52 +53,53 @@ A.declare("cf_kv_validate_evict_desc", A.I32, [A.P])
 A.declare("cf_kv_evict_groups_async", A.I32, [A.P, A.P])
 
 
-def _need(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> torch.Tensor:
+def _need(t: torch.Tensor, name: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
     """The C calls see addresses only: what a tensor has to be is checked here."""
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous {dtype} tensor of shape {tuple(shape)} on {device} is needed, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _on(device: torch.device, stream):
-    """The stream of a call, which has to belong to the tensors' device."""
-    stream = stream if stream is not None else torch.cuda.current_stream(device)
-    if device.type == "cuda" and stream.device != device:
+def _raw_stream(device: torch.device, stream) -> int:
+    """Handle of `stream` (default: the device's current stream), which has to belong to the tensors' device."""
+    if stream is None:
+        # torch.cuda.current_stream(device).cuda_stream without the Stream object, whose making takes 2 us of a 7 us call
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    if stream.device != device:
         raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-    return stream
+    return stream.cuda_stream
 
 
-def _call(name: str, device: torch.device, stream, *args) -> None:
+def _call(name: str, device: torch.device, s: int, *args) -> None:
     """One asynchronous C call with the tensors' device as the current one."""
-    s = _on(device, stream)
     fn = getattr(A.lib(), name)
-    if device.type == "cuda" and device.index is not None and device.index != torch.cuda.current_device():
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            A.check(fn(*args, s.cuda_stream), name)
+            A.check(fn(*args, s), name)
     else:
-        A.check(fn(*args, s.cuda_stream), name)
+        A.check(fn(*args, s), name)
 
 
-def _with_workspace(desc, need: int, device: torch.device, stream, holder=None) -> None:
-    """Gives `holder` (the descriptor by default) a workspace for calls on `stream`, allocated for that stream."""
+def _with_workspace(desc, need: int, device: torch.device, stream) -> None:
+    """Gives the descriptor a workspace for calls on `stream`, allocated for that stream."""
     if need:
-        kv._give_workspace(desc if holder is None else holder, need, device, _on(device, stream))
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        with torch.cuda.device(device):
+            kv._give_workspace(desc, need, device, stream if stream is not None else torch.cuda.current_stream(device))
 
 
-def _for_stream(desc, holder, cls, device, stream):
-    """`holder`, or a copy with a workspace of its own where it was made for another stream."""
-    s = _on(device, stream)
-    if holder.workspace and getattr(holder, "workspace_stream", s.cuda_stream) != s.cuda_stream:
-        copy = cls.from_buffer_copy(holder)
-        copy.held = getattr(holder, "held", None)
-        kv._give_workspace(copy, copy.workspace_bytes, device, s)
+def _for_stream(d, cls, device: torch.device, stream, s: int):
+    """The descriptor, or a copy with a workspace of its own where it was made for another stream than s."""
+    if d.workspace and d.workspace_stream != s:
+        copy = cls.from_buffer_copy(d)
+        _with_workspace(copy, d.workspace_bytes, device, stream)
         return copy
-    return holder
+    return d
 
 
 # ---------------------------------------------------------------------------------------------------- key bounds
@@ -128,10 +129,11 @@ def key_bounds(keys: torch.Tensor, first_page: torch.Tensor, page_counts: torch.
         _need(token_counts, "token_counts", torch.int32, (keys.shape[0],), dev)
     if slots is not None:
         _need(slots, "slots", torch.int64, (n,), dev)
-    _need(out.scales, "out.scales", torch.float32, out.scales.shape, dev)
-    _need(out.codes, "out.codes", torch.int8, (*out.scales.shape, 2 * D), dev)
+    rows = out.scales.shape
+    _need(out.scales, "out.scales", torch.float32, rows, dev)
+    _need(out.codes, "out.codes", torch.int8, (*rows, 2 * D), dev)
     if n:
-        _call("cf_kv_key_bounds_async", dev, stream, keys.data_ptr(), n, first_page.data_ptr(), page_counts.data_ptr(),
+        _call("cf_kv_key_bounds_async", dev, _raw_stream(dev, stream), keys.data_ptr(), n, first_page.data_ptr(), page_counts.data_ptr(),
               _ptr(token_counts), D, _ptr(slots), out.codes.data_ptr(), out.scales.data_ptr(), out.scales.numel())
     return out
 
@@ -190,8 +192,8 @@ def select(kvb: kv.BatchedKv, bounds: KeyBounds, queries: torch.Tensor, query_po
     [seq_count, query_heads, D] is largest, the first keep_first and the last keep_last always, ascending, then NO_UNIT."""
     d = desc if desc is not None else select_desc(kvb, bounds, queries, query_pos, units, unit_groups, keep_first, keep_last, stream)
     dev = kvb.group_offsets.device
-    d = _for_stream(d, d, cf_kv_select_desc, dev, stream)
-    _call("cf_kv_select_groups_async", dev, stream, C.byref(d))
+    s = _raw_stream(dev, stream)
+    _call("cf_kv_select_groups_async", dev, s, C.byref(_for_stream(d, cf_kv_select_desc, dev, stream, s)))
     return units
 
 
@@ -235,9 +237,9 @@ def attention(kvb: kv.BatchedKv, queries: torch.Tensor, output: torch.Tensor, qu
     dev = kvb.group_offsets.device
     d = desc if desc is not None else attention_desc(kvb, queries, output, query_pos, softmax_scale, units, unit_groups, weights,
                                                      weights_out, decay, splits, stream)
-    sel = d.selection
-    d = _for_stream(d, d, kv.cf_kv_batched_desc, dev, stream)
-    _call("cf_kv_paged_attention_selected_async", dev, stream, C.byref(d), C.byref(sel))
+    s = _raw_stream(dev, stream)
+    _call("cf_kv_paged_attention_selected_async", dev, s, C.byref(_for_stream(d, kv.cf_kv_batched_desc, dev, stream, s)),
+          C.byref(d.selection))
 
 
 # ---------------------------------------------------------------------------------------------------- eviction
@@ -289,4 +291,5 @@ def evict(kvb: kv.BatchedKv, weights: torch.Tensor, budget_units: int, out: Evic
     keep_last, then those of the largest accumulated `weights`. out=None evicts in place: kvb's tables and lengths, weights
     and bounds."""
     d = desc if desc is not None else evict_desc(kvb, weights, budget_units, out, bounds, unit_groups, keep_first, keep_last)
-    _call("cf_kv_evict_groups_async", kvb.group_offsets.device, stream, C.byref(d))
+    dev = kvb.group_offsets.device
+    _call("cf_kv_evict_groups_async", dev, _raw_stream(dev, stream), C.byref(d))
