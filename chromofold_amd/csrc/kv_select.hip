@@ -352,8 +352,6 @@ int row_threads(const cf_kv_select_desc *d) {
 }
 
 // ---- eviction ---------------------------------------------------------------------------------------------------
-constexpr int kEvictThreads = 256;
-
 struct Budget {
   uint32_t tokens, groups, units, kept;
   __device__ Budget(const cf_kv_evict_desc &d, uint32_t t) {
@@ -370,81 +368,84 @@ __global__ void evict_tokens_kernel(cf_kv_evict_desc d) {
   if (s < d.seq_count) d.seq_tokens_out[s] = Budget(d, d.seq_tokens[s]).tokens_out(d);
 }
 
-// One workgroup per (KV head, sequence). Units are decided and moved in rounds of kEvictThreads of them in index order: a
+constexpr uint32_t kEvictKeys = 8192;  // keys of a row that are held in LDS; longer rows read their weights again
+
+// One workgroup of T threads per (KV head, sequence). Units are decided and moved in rounds of T of them in index order: a
 // kept unit moves down or stays, so a round's destinations lie at or before its sources and before every later round's;
-// within a round all reads come before the first write. That is what makes eviction in place safe.
-template <int D>
-__global__ __launch_bounds__(kEvictThreads) void evict_kernel(cf_kv_evict_desc d, bool tokens_here) {
-  __shared__ cfsel::TopkShared<kEvictThreads> sh;
-  __shared__ uint32_t s_from[2 * kEvictThreads];  // source groups of the round's kept groups
+// within a step all reads come before the first write. That is what makes eviction in place safe. Bound by latency: the
+// weights, the pick, then one read and one write of everything a step moves.
+template <int D, int T>
+__global__ __launch_bounds__(T) void evict_kernel(cf_kv_evict_desc d, bool tokens_here) {
+  constexpr uint32_t kL = 2 * D / 16;       // 16-byte pieces of a record
+  constexpr uint32_t kPer = 8;              // pieces a thread moves in a step
+  constexpr uint32_t kStep = T * kPer / kL; // groups of a step
+  __shared__ cfsel::TopkShared<T> sh;
+  __shared__ uint32_t s_from[2 * T];  // source groups of the round's kept groups
+  __shared__ uint32_t s_key[kEvictKeys];
   const uint32_t head = blockIdx.x, seq = blockIdx.y, unit = d.unit_groups;
   const uint32_t tid = threadIdx.x;
   const Budget b(d, d.seq_tokens[seq]);
   const size_t row = (static_cast<size_t>(seq) * d.kv_head_count + head) * d.max_groups;
   const float *w = d.weights + row;
   const uint32_t *off = d.group_offsets + row;
-  uint32_t *off_out = d.group_offsets_out + row;
-  auto wait_loads = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
-
-  auto key = [&](uint32_t u) {
+  auto key_of = [&](uint32_t u) {
     float x = w[u * unit];
     if (unit == 2 && 2 * u + 1 < b.groups) x += w[2 * u + 1];
     return cfsel::sortable(x);
   };
-  cfsel::take_largest<kEvictThreads>(
-      key, b.units, d.keep_first, d.keep_last, b.kept, sh,
+  const bool held = b.units <= kEvictKeys;
+  if (held && b.units > b.kept) {
+    for (uint32_t u = tid; u < b.units; u += T) s_key[u] = key_of(u);
+    __syncthreads();
+  }
+  cfsel::take_largest<T>(
+      [&](uint32_t u) { return held ? s_key[u] : key_of(u); }, b.units, d.keep_first, d.keep_last, b.kept, sh,
       [&](uint32_t u, bool take, uint32_t pos) {
         for (uint32_t j = 0; j < unit; ++j) {
           const uint32_t g = u * unit + j;
           if (take) {
-            if (g < b.groups) s_from[(pos * unit + j) % (2 * kEvictThreads)] = g;
+            if (g < b.groups) s_from[(pos * unit + j) % (2 * T)] = g;
           } else if (d.dropped) {
             d.dropped[row + pos * unit + j] = off[g];  // a dropped unit is not the last: all its groups exist
           }
         }
       },
-      [&](uint32_t base, uint32_t before, uint32_t cnt) {
+      [&](uint32_t, uint32_t before, uint32_t cnt) {
         // kept groups [g0, g1) of the round; s_from is read at the same positions modulo its size
         const uint32_t g0 = before * unit, g1 = min((before + cnt) * unit, b.groups - (b.units - b.kept) * unit);
         __syncthreads();
-        for (uint32_t a = g0; a < g1; a += kEvictThreads) {  // (two steps for pairs)
-          const uint32_t i = a + tid;
-          const bool in = i < g1;
-          const uint32_t src = in ? s_from[i % (2 * kEvictThreads)] : 0u;
+        for (uint32_t a = g0; a < g1; a += kStep) {
+          const uint32_t i = a + tid, m = min(g1 - a, kStep) * kL;
+          const bool in = tid < kStep && i < g1;
           uint32_t o = 0;
           float x = 0.0f, sc = 0.0f;
+          int4_t v[kPer];
           if (in) {
+            const uint32_t src = s_from[i % (2 * T)];
             o = off[src];
             if (d.weights_out) x = w[src];
             if (d.codes_out) sc = d.scales[row + src];
           }
-          wait_loads();
+          if (d.codes_out) {
+#pragma unroll
+            for (uint32_t e = 0; e < kPer; ++e) {
+              const uint32_t p = e * T + tid;
+              if (p < m)
+                v[e] = *reinterpret_cast<const int4_t *>(d.codes + (row + s_from[(a + p / kL) % (2 * T)]) * (2 * D) + 16 * (p % kL));
+            }
+          }
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every read of this wavefront has returned
           __syncthreads();
           if (in) {
-            off_out[i] = o;
+            d.group_offsets_out[row + i] = o;
             if (d.weights_out) d.weights_out[row + i] = x;
             if (d.codes_out) d.scales_out[row + i] = sc;
           }
           if (d.codes_out) {
-            constexpr uint32_t kL = 2 * D / 16;  // 16-byte pieces of a record
-            constexpr uint32_t kPer = 8;         // pieces a thread moves at a time
-            const uint32_t m = min(g1 - a, static_cast<uint32_t>(kEvictThreads)) * kL;
-            for (uint32_t p0 = 0; p0 < m; p0 += kPer * kEvictThreads) {
-              int4_t v[kPer];
 #pragma unroll
-              for (uint32_t e = 0; e < kPer; ++e) {
-                const uint32_t p = p0 + e * kEvictThreads + tid;
-                if (p < m)
-                  v[e] = *reinterpret_cast<const int4_t *>(d.codes + (row + s_from[(a + p / kL) % (2 * kEvictThreads)]) * (2 * D) +
-                                                           16 * (p % kL));
-              }
-              wait_loads();
-              __syncthreads();
-#pragma unroll
-              for (uint32_t e = 0; e < kPer; ++e) {
-                const uint32_t p = p0 + e * kEvictThreads + tid;
-                if (p < m) *reinterpret_cast<int4_t *>(d.codes_out + (row + a + p / kL) * (2 * D) + 16 * (p % kL)) = v[e];
-              }
+            for (uint32_t e = 0; e < kPer; ++e) {
+              const uint32_t p = e * T + tid;
+              if (p < m) *reinterpret_cast<int4_t *>(d.codes_out + (row + a + p / kL) * (2 * D) + 16 * (p % kL)) = v[e];
             }
           }
         }
@@ -453,10 +454,17 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(cf_kv_evict_desc d
   const uint32_t left = b.groups - (b.units - b.kept) * unit, gone = b.groups - left;
   __syncthreads();  // every weight has been read
   if (d.weights_out)
-    for (uint32_t i = left + tid; i < d.max_groups; i += kEvictThreads) d.weights_out[row + i] = 0.0f;
+    for (uint32_t i = left + tid; i < d.max_groups; i += T) d.weights_out[row + i] = 0.0f;
   if (d.dropped)
-    for (uint32_t i = gone + tid; i < d.max_groups; i += kEvictThreads) d.dropped[row + i] = CF_KV_NO_UNIT;
+    for (uint32_t i = gone + tid; i < d.max_groups; i += T) d.dropped[row + i] = CF_KV_NO_UNIT;
   if (tokens_here && head == 0 && tid == 0) d.seq_tokens_out[seq] = b.tokens_out(d);
+}
+
+template <int D>
+void launch_evict(const cf_kv_evict_desc &d, bool tokens_here, hipStream_t s) {
+  const dim3 grid(d.kv_head_count, d.seq_count);
+  if (d.max_groups / d.unit_groups <= 256) evict_kernel<D, 256><<<grid, 256, 0, s>>>(d, tokens_here);
+  else evict_kernel<D, 1024><<<grid, 1024, 0, s>>>(d, tokens_here);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -551,9 +559,8 @@ extern "C" cf_status cf_kv_evict_groups_async(const cf_kv_evict_desc *d, void *s
   const hipStream_t s = cfd::as_stream(stream);
   // in place, the lengths are still read by the workgroups of the other heads: a launch of their own behind them
   const bool tokens_here = d->seq_tokens_out != d->seq_tokens;
-  const dim3 grid(d->kv_head_count, d->seq_count);
-  if (d->head_dim == 128) evict_kernel<128><<<grid, kEvictThreads, 0, s>>>(*d, tokens_here);
-  else evict_kernel<64><<<grid, kEvictThreads, 0, s>>>(*d, tokens_here);
+  if (d->head_dim == 128) launch_evict<128>(*d, tokens_here, s);
+  else launch_evict<64>(*d, tokens_here, s);
   if (!tokens_here) evict_tokens_kernel<<<cfd::grid_for(d->seq_count, 256), 256, 0, s>>>(*d);
   return cfd::launch_status();
 }
