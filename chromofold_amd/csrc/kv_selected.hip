@@ -4,8 +4,9 @@
 // Per (sequence, KV head), over the tokens t of the listed groups, query heads h of the KV head:
 //   s_ht = scale q_h . (ks_page (sym - 128)_t),  p = softmax_t(s),  o_h = sum_t p_ht vs_page (sym - 128)_t,
 //   weights_out[g] = decay weights_in[g] + sum_h sum_{t in g} p_ht.
-// One pass over the blobs with a running maximum and sum per wavefront; wavefronts are joined in LDS, workgroups by a second
-// small launch, which also turns the groups' (maximum, sum) pairs into weights.
+// One pass over the blobs with a running maximum and sum per wavefront; a row's states are joined in LDS or by a second small
+// launch, which also turns the groups' (maximum, sum) pairs into weights. Bound by reading the blobs: 32 x 512 groups of all
+// 8 heads (2.16 GB) at 6.3 TB/s with that launch, 6.7 as one workgroup per row.
 //
 // A wavefront takes one 64-token group (16.4 KB at D = 128) at a time, both products on v_mfma_f32_16x16x32_f16 with the 16
 // rows = query heads, so up to 16 of them cost what one does:
@@ -26,6 +27,7 @@
 
 #include "cf_device.hpp"
 #include "chromofold/kv_select.h"
+#include "kv_topk.hpp"
 
 namespace {
 
@@ -37,21 +39,33 @@ typedef float float4a4_t __attribute__((ext_vector_type(4), aligned(4)));  // qu
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kHdr = 64;
-constexpr int kWaves = 4;     // of a workgroup that takes part of a row
+constexpr int kWaves = 4;     // of a workgroup
 constexpr int kWavesRow = 8;  // of a workgroup that takes a whole row
+constexpr uint32_t kResident = 8;  // wavefronts of a CU at these kernels' registers
 constexpr int kRows = 16;
 constexpr int kPStride = 80;  // halves of a row of the weight tile: the four rows a store instruction writes start 32 banks apart
 constexpr uint32_t kRowStats = 2048;  // group statistics that a workgroup with a whole row holds in LDS
+constexpr uint32_t kSpanSeqs = 1024;  // sequences of a span launch (their prefix sums are made by each workgroup)
 constexpr float kLog2e = 1.44269504088896340736f;
+
+// How a launch cuts the rows ((sequence, KV head) pairs, each of some slots: list entries, or groups without a list):
+//   kSpan   all rows' slots laid end to end, heads outermost, an equal stretch for each wavefront. The lengths are device
+//           memory: a grid over rows is sized for the longest sequence and waits for it, a stretch is equal whatever they are,
+//           and a wavefront's loads run on from one row into the next.
+//   kRow    a workgroup per row, which finishes it: no second launch
+//   kSplit  `splits` workgroups per row, `per` slots each: a row's result depends on its own sequence alone
+enum Mode { kSpan, kRow, kSplit };
 
 struct SelArgs {
   cf_kv_batched_desc d;
   cf_kv_selection s;
   uint32_t slots;    // the most slots of a row: max_units * unit_groups list entries, or max_groups without a list
-  uint32_t splits;   // workgroups of a row
-  uint32_t per;      // slots of a workgroup
-  float *sums;       // [row][split][gqa][D]: sum of p v
-  float2 *states;    // [row][split][gqa]: maximum (log2 units) and sum of p
+  uint32_t splits;   // kSplit: workgroups of a row
+  uint32_t per;      // kSplit: slots of a workgroup
+  uint32_t nwaves;   // kSpan: wavefronts
+  uint32_t *pre;     // kSpan: [seq_count + 1] prefix sums of the sequences' slots, for the second launch
+  float *sums;       // [state][gqa][D]: sum of p v
+  float2 *states;    // [state][gqa]: maximum (log2 units) and sum of p
   float2 *stats;     // [row][slot][gqa]: a group's maximum (log2 units) and sum of exp2(score - maximum)
 };
 
@@ -128,15 +142,263 @@ __device__ __forceinline__ void write_weights(const SelArgs &a, size_t row, cons
   }
 }
 
-// ROW: the workgroup has the row to itself and finishes it; its groups' statistics stay in LDS.
+// One group's blob on its way: K quads, V quads and the header's fields of this lane's page.
+template <int D>
+struct Blob {
+  uint4_t kw[D / 16];
+  uint32_t vw[D / 4];
+  float ks, vs;
+  uint32_t tc, codec, dim;
+  __device__ __forceinline__ void load_k(const uint8_t *p) {
+    const int lane = threadIdx.x & 63, n = lane & 15;
+    codec = *reinterpret_cast<const uint32_t *>(p);
+    dim = *reinterpret_cast<const uint16_t *>(p + 20);
+    tc = reinterpret_cast<const uint16_t *>(p + 12)[n >> 2];
+    ks = reinterpret_cast<const float *>(p + 32)[n >> 2];
+    vs = reinterpret_cast<const float *>(p + 48)[n >> 2];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      kw[i] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t *>(p + kHdr) + 64 * i + lane);
+  }
+  __device__ __forceinline__ void load_v(const uint8_t *p) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i)
+      vw[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p + kHdr + 64 * D) + 64 * i + lane);
+  }
+};
+
+// A wavefront's LDS: the weight tile, and statistics of the groups looked up together, on their way to memory in whole
+// lines (one group's are 8 bytes a head; written on their own they cost 256 rows of 512 groups 15 of 350 us).
+constexpr uint32_t kLookStats = 256;
+struct WaveLds {
+  _Float16 p[2][kRows][kPStride];
+  float2 stat[kLookStats];
+};
+__device__ __forceinline__ uint32_t look_slots(uint32_t gqa) { return min(64u, kLookStats / gqa); }
+
+// Queries of one row as they lie in memory, in the layout of the A operands: row n, dims 4 (8 s + b) .. + 3 and
+// 4 (8 s + 4 + b) .. + 3 of step s.
+template <int D>
+struct Query {
+  float4_t x[D / 16];
+  __device__ __forceinline__ void load(const SelArgs &a, uint32_t seq, uint32_t head, uint32_t gqa) {
+    const int lane = threadIdx.x & 63, n = lane & 15, b = lane >> 4;
+    const float *q = a.d.queries +
+                     (static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + min(static_cast<uint32_t>(n), gqa - 1)) * D;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) x[s] = *reinterpret_cast<const float4a4_t *>(q + 4 * (4 * s + b));
+  }
+};
+
+// A wavefront's running state of one row: maximum and sum of the heads 4 b + r, sums of p v of the heads 4 b + r (row r of the
+// accumulators) at dim 16 i + n.
+template <int D>
+struct RowState {
+  float m[4], l[4];
+  int e;  // acc holds sums in units of 2^e
+  float4_t acc[D / 16];
+  float unit[4];  // log2-unit factor of the heads' scores, without the page's scale
+  half8_t qh[D / 32], ql[D / 32];
+  bool bad;
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m[r] = -INFINITY, l[r] = 0.0f;
+    e = -(1 << 20);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) acc[i] = float4_t{0, 0, 0, 0};
+    bad = false;
+  }
+
+  // Each head in units of a power of two that puts its largest element into [2^14, 2^15), as f16 hi + lo.
+  __device__ __forceinline__ void set_query(const SelArgs &a, const Query<D> &q, uint32_t gqa) {
+    const int lane = threadIdx.x & 63, n = lane & 15, b = lane >> 4;
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(q.x[s][j]));
+    top = cfd::rows4_max(top);
+    const int x = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
+    const float u = ldexpf(a.d.softmax_scale * kLog2e, x);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) unit[r] = __shfl(u, 4 * b + r);
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = static_cast<uint32_t>(n) < gqa ? ldexpf(q.x[2 * s + j / 4][j % 4], -x) : 0.0f;
+        _Float16 hi, lo;
+        cfd::split_mul_f16(v, 1.0f, hi, lo);
+        qh[s][j] = hi;
+        ql[s][j] = lo;
+      }
+  }
+
+  // Group g (its K and V in w). next: the blob to load after it, or null. put(h, m, l) receives its statistics if `stats`.
+  template <typename Put>
+  __device__ __forceinline__ void attend(Blob<D> &w, uint32_t g, uint32_t visible, uint32_t gqa, WaveLds &lds,
+                                         const uint8_t *next, bool stats, const Put &put) {
+    constexpr int kTiles = D / 16;
+    const int lane = threadIdx.x & 63, n = lane & 15, b = lane >> 4;
+    // ---- scores of the tokens 4 n + i (one page per lane) for the heads 4 b + r
+    float4_t sc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc[i] = float4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      half8_t k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = signed_half8(w.kw[2 * s][i], w.kw[2 * s + 1][i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[s], k[i], sc[i], 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[s], k[i], sc[i], 0, 0, 0);
+    }
+    bad |= w.codec != CF_KV_CODEC_INT8 || w.dim != D;
+    // tokens of a page are visible from its first on
+    const uint32_t page = 64 * g + 16 * (n >> 2), first = 64 * g + 4 * n, end = min(page + min(w.tc, 16u), visible);
+    const uint32_t nvis = end > first ? min(end - first, 4u) : 0u;
+    const bool page_vis = w.tc > 0 && page < visible;
+    const float ks = w.ks, vs = w.vs;
+    if (next) w.load_k(next);
+    // ---- online softmax
+    float mx[4], p[4][4], sum[4];
+    bool moved = false;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float f = unit[r] * ks;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i][r] = static_cast<uint32_t>(i) < nvis ? sc[i][r] * f : -INFINITY;
+      mx[r] = fmaxf(fmaxf(p[0][r], p[1][r]), fmaxf(p[2][r], p[3][r]));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      mx[r] = cfd::row16_max(mx[r]);
+      moved |= mx[r] > m[r];
+    }
+    // units of the P.V sums: the exponent of the group's largest V scale among its visible pages, less 15, so that
+    // weights p vs lie in [0, 2^15) and those down to 2^-29 of that are normal f16 numbers. Sums move to a larger unit
+    // at once and to a smaller one when 2^8 below (a factor of a power of two; clamped so that it cannot overflow).
+    constexpr int kNone = -(1 << 24);
+    const int ep = page_vis ? __builtin_amdgcn_frexp_expf(vs) - 15 : kNone;
+    const int eb = max(max(__builtin_amdgcn_readlane(ep, 0), __builtin_amdgcn_readlane(ep, 4)),
+                       max(__builtin_amdgcn_readlane(ep, 8), __builtin_amdgcn_readlane(ep, 12)));
+    int e_new = e;
+    if (eb != kNone && (eb > e || eb < e - 8)) e_new = max(eb, e - 60);
+    if (__builtin_amdgcn_ballot_w64(moved) || e_new != e) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float mn = fmaxf(m[r], mx[r]);
+        const float al = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - mn);
+        m[r] = mn;
+        l[r] *= al;
+        const float f = ldexpf(al, max(e - e_new, -200));  // 0 before the first visible token
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) acc[i][r] *= f;
+      }
+      e = e_new;
+    }
+    const float vsn = page_vis ? ldexpf(vs, -e) : 0.0f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float m0 = m[r] == -INFINITY ? 0.0f : m[r];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i][r] = __builtin_amdgcn_exp2f(p[i][r] - m0);  // exp2(-inf) = 0
+      sum[r] = (p[0][r] + p[1][r]) + (p[2][r] + p[3][r]);
+      l[r] += sum[r];
+    }
+    if (stats) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float t = cfd::row16_sum(sum[r]);
+        if (n == r && static_cast<uint32_t>(4 * b + r) < gqa) put(4 * b + r, m[r], t);
+      }
+    }
+    if (static_cast<uint32_t>(4 * b) < gqa) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        _Float16 h0, l0, h1, l1, h2, l2, h3, l3;
+        cfd::split2_mul_f16(p[0][r], p[1][r], vsn, h0, l0, h1, l1);
+        cfd::split2_mul_f16(p[2][r], p[3][r], vsn, h2, l2, h3, l3);
+        *reinterpret_cast<half4_t *>(&lds.p[0][4 * b + r][4 * n]) = half4_t{h0, h1, h2, h3};
+        *reinterpret_cast<half4_t *>(&lds.p[1][4 * b + r][4 * n]) = half4_t{l0, l1, l2, l3};
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    // ---- P.V: k-values of lane group b = tokens 8 tp .. 8 tp + 7 of page b
+#pragma unroll
+    for (int tp = 0; tp < 2; ++tp) {
+      const half8_t ph = *reinterpret_cast<const half8_t *>(&lds.p[0][n][16 * b + 8 * tp]);
+      const half8_t pl = *reinterpret_cast<const half8_t *>(&lds.p[1][n][16 * b + 8 * tp]);
+#pragma unroll
+      for (int i0 = 0; i0 < kTiles; i0 += 4) {
+        half8_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = signed_half8(w.vw[2 * tp * kTiles + i0 + i], w.vw[(2 * tp + 1) * kTiles + i0 + i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, v[i], acc[i0 + i], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, v[i], acc[i0 + i], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (next) w.load_v(next);
+  }
+
+  // l becomes the sum over all lanes; m a NaN where the row is broken or holds one (a NaN score leaves the maximum as it was
+  // and makes the sum a NaN).
+  __device__ __forceinline__ void close() {
+    const bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      l[r] = cfd::row16_sum(l[r]);
+      if (broken || l[r] != l[r]) m[r] = __builtin_nanf("");
+    }
+  }
+
+  // The closed state to memory, its sums in absolute units.
+  __device__ __forceinline__ void store(float *sums, float2 *states, uint32_t gqa) const {
+    const int lane = threadIdx.x & 63, n = lane & 15, b = lane >> 4;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (static_cast<uint32_t>(4 * b + r) < gqa) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) sums[(4 * b + r) * D + 16 * i + n] = ldexpf(acc[i][r], max(e, -200));
+        if (n == 0) states[4 * b + r] = float2{m[r], l[r]};
+      }
+  }
+};
+
+__device__ __forceinline__ const uint8_t *blob_at(const SelArgs &a, uint32_t offsets, int lane) {
+  // (readlane returns an int: offsets from 2^31 on must not be sign-extended)
+  return a.d.pool + static_cast<size_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(offsets, lane))) * 16;
+}
+
+// Statistics of `count` slots looked up together from the wavefront's LDS to memory; `dest`: the place of this lane's slot.
+__device__ __forceinline__ void write_stats(float2 *__restrict__ to, const WaveLds &lds, uint32_t dest, uint32_t count, uint32_t gqa) {
+  const uint32_t lane = threadIdx.x & 63;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  for (uint32_t e0 = 0; e0 < count * gqa; e0 += 64) {
+    const uint32_t e = e0 + lane, i = min(e / gqa, 63u);
+    const size_t at = __shfl(dest, static_cast<int>(i));
+    if (e < count * gqa) to[at * gqa + (e - i * gqa)] = lds.stat[e];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// kRow and kSplit: a workgroup takes slots of one row, its wavefronts a block of them each.
 template <int D, int W, bool ROW>
-__global__ __launch_bounds__(64 * W, 2) void selected_kernel(SelArgs a) {
-  constexpr int kSteps = D / 32;   // k-steps of q . k
-  constexpr int kTiles = D / 16;   // dim tiles of p . v
-  constexpr int kKLoads = D / 16;  // 16-byte loads of a lane: K
-  constexpr int kVLoads = D / 4;   // 4-byte loads of a lane: V
+__global__ __launch_bounds__(64 * W, 2) void row_kernel(SelArgs a) {
   __shared__ union {
-    _Float16 p[W][2][kRows][kPStride];
+    WaveLds wave[W];
     float red[W][kRows][D];
   } sh;
   __shared__ float s_m[W][kRows], s_l[W][kRows];
@@ -145,244 +407,79 @@ __global__ __launch_bounds__(64 * W, 2) void selected_kernel(SelArgs a) {
 
   const int lane = threadIdx.x & 63, n = lane & 15, b = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t split = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
+  const uint32_t head = blockIdx.y, seq = blockIdx.z;
   const uint32_t gqa = a.d.query_head_count / a.d.kv_head_count;
   const size_t row = static_cast<size_t>(seq) * a.d.kv_head_count + head;
+  // Workgroups go to the 8 dies in turn: with a multiple of 8 splits a die would take the same splits of every row, and the
+  // last ones are empty in short rows (32 x 500-32768 tokens in 8 splits: 278 us, rotated 222).
+  const uint32_t split = ROW ? 0 : (blockIdx.x + static_cast<uint32_t>(row % a.splits)) % a.splits;
   const uint32_t *list = a.s.units ? a.s.units + row * a.s.max_units : nullptr;
   const uint32_t *grow = a.d.group_offsets + row * a.d.max_groups;
-  auto put_stat = [&](uint32_t slot, uint32_t h, float m, float l) {
-    if constexpr (ROW) s_stat[slot * gqa + h] = float2{m, l};
-    else a.stats[(row * a.slots + slot) * gqa + h] = float2{m, l};
-  };
-
-  // ---- queries, straight from memory into the layout of the A operands: row n, dims 4 (8 s + b) .. + 3 and
-  // 4 (8 s + 4 + b) .. + 3 of step s. Their loads come first, so that they are there when the list entry and the offset,
-  // which the first group waits for anyway, have come.
-  const float *qrow = a.d.queries + (static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + min(static_cast<uint32_t>(n), gqa - 1)) * D;
-  float4_t qx[2 * kSteps];
-#pragma unroll
-  for (int s = 0; s < 2 * kSteps; ++s) qx[s] = *reinterpret_cast<const float4a4_t *>(qrow + 4 * (4 * s + b));
-
+  // The queries' loads come first, so that they are there when the list entry and the offset, which the first group waits
+  // for anyway, have come.
+  Query<D> q;
+  q.load(a, seq, head, gqa);
   const uint32_t visible = visible_tokens(a.d.seq_tokens[seq], a.d.query_pos[seq], a.d.max_groups);
   const uint32_t ngroups = (visible + 63) / 64, nslots = row_slots(a, ngroups);
   const uint32_t s0 = ROW ? 0 : min(split * a.per, nslots), s1 = ROW ? nslots : min(nslots, s0 + a.per);
-
-  half8_t qh[kSteps], ql[kSteps];
-  float unit[4];  // log2-unit factor of the rows' scores, without the page's scale
-  // each head in units of a power of two that puts its largest element into [2^14, 2^15)
-  auto split_queries = [&] {
-    float top = 0.0f;
-#pragma unroll
-    for (int s = 0; s < 2 * kSteps; ++s)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(qx[s][j]));
-    top = cfd::rows4_max(top);
-    const int e = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
-    const float u = ldexpf(a.d.softmax_scale * kLog2e, e);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) unit[r] = __shfl(u, 4 * b + r);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = static_cast<uint32_t>(n) < gqa ? ldexpf(qx[2 * s + j / 4][j % 4], -e) : 0.0f;
-        _Float16 hi, lo;
-        cfd::split_mul_f16(x, 1.0f, hi, lo);
-        qh[s][j] = hi;
-        ql[s][j] = lo;
-      }
-  };
-
-  float m_run[4], l_run[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) m_run[r] = -INFINITY, l_run[r] = 0.0f;
-  int e_run = -(1 << 20);  // acc holds sums in units of 2^e_run
-  float4_t acc[kTiles];
-#pragma unroll
-  for (int i = 0; i < kTiles; ++i) acc[i] = float4_t{0, 0, 0, 0};
-  bool bad = false, split_done = false;
-
-  // The wavefront's slots s0 + wave, + W, ...: 64 of them at a time, one a lane, so that no load of the loop below
-  // waits for a list entry or an offset.
-  for (uint32_t c0 = s0 + wave; c0 < s1; c0 += 64 * W) {
-    const uint32_t mine = c0 + lane * W;
+  RowState<D> st;
+  st.reset();
+  bool split_done = false, bad = false;
+  // Slots are looked up 64 at a time (fewer where that many statistics would not fit), one a lane, so that no load of the
+  // loop below waits for a list entry or an offset.
+  const uint32_t pw = (s1 - s0 + W - 1) / W, w0 = min(s1, s0 + wave * pw), w1 = min(s1, w0 + pw);
+  const uint32_t step = ROW ? 64u : look_slots(gqa);
+  const bool stats = a.s.weights_out != nullptr;
+  WaveLds &lds = sh.wave[wave];
+  for (uint32_t c0 = w0; c0 < w1; c0 += step) {
+    const uint32_t mine = c0 + lane;
+    float2 *stat = ROW ? s_stat + c0 * gqa : lds.stat;
     uint32_t g_l = 0xFFFFFFFFu, off_l = 0;
-    if (mine < s1) {
+    const bool in = mine < w1 && static_cast<uint32_t>(lane) < step;
+    if (in) {
       g_l = listed_group(a, list, mine, bad);
       if (g_l < ngroups) off_l = grow[g_l];
     }
     const bool here = g_l < ngroups;
     uint64_t todo = __builtin_amdgcn_ballot_w64(here);
-    if (a.s.weights_out && mine < s1 && !here)
-      for (uint32_t h = 0; h < gqa; ++h) put_stat(mine, h, -INFINITY, 0.0f);
-    if (!todo) continue;
-
-    uint4_t kw[kKLoads];
-    uint32_t vw[kVLoads];
-    float ks, vs;
-    uint32_t tc, codec, dim;
-    auto blob_of = [&](int i) {  // (readlane returns an int: offsets from 2^31 on must not be sign-extended)
-      return a.d.pool + static_cast<size_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(off_l, i))) * 16;
-    };
-    auto load_k = [&](const uint8_t *p) {
-      codec = *reinterpret_cast<const uint32_t *>(p);
-      dim = *reinterpret_cast<const uint16_t *>(p + 20);
-      tc = reinterpret_cast<const uint16_t *>(p + 12)[n >> 2];
-      ks = reinterpret_cast<const float *>(p + 32)[n >> 2];
-      vs = reinterpret_cast<const float *>(p + 48)[n >> 2];
-#pragma unroll
-      for (int i = 0; i < kKLoads; ++i)
-        kw[i] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t *>(p + kHdr) + 64 * i + lane);
-    };
-    auto load_v = [&](const uint8_t *p) {
-#pragma unroll
-      for (int i = 0; i < kVLoads; ++i)
-        vw[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p + kHdr + 64 * D) + 64 * i + lane);
-    };
-    int cur = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    const uint8_t *blob = blob_of(cur);
-    load_k(blob);
-    load_v(blob);
-    if (!split_done) split_queries();
-    split_done = true;
-    for (;;) {
-      const int next = todo ? __builtin_ctzll(todo) : -1;
-      todo &= todo - 1;
-      const uint32_t g = __builtin_amdgcn_readlane(g_l, cur);
-      const uint8_t *blob_next = next >= 0 ? blob_of(next) : blob;
-      // ---- scores of the tokens 4 n + i (one page per lane) for the heads 4 b + r
-      float4_t sc[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[i] = float4_t{0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        half8_t k[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = signed_half8(kw[2 * s][i], kw[2 * s + 1][i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[s], k[i], sc[i], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[s], k[i], sc[i], 0, 0, 0);
+    if (stats && in && !here)
+      for (uint32_t h = 0; h < gqa; ++h) stat[lane * gqa + h] = float2{-INFINITY, 0.0f};
+    if (todo) {
+      int cur = __builtin_ctzll(todo);
+      Blob<D> w;
+      w.load_k(blob_at(a, off_l, cur));
+      w.load_v(blob_at(a, off_l, cur));
+      if (!split_done) st.set_query(a, q, gqa);
+      split_done = true;
+      for (;;) {
+        todo &= todo - 1;
+        const int next = todo ? __builtin_ctzll(todo) : -1;
+        const uint32_t g = static_cast<uint32_t>(__builtin_amdgcn_readlane(g_l, cur));
+        float2 *put = stat + static_cast<uint32_t>(cur) * gqa;
+        st.attend(w, g, visible, gqa, lds, next >= 0 ? blob_at(a, off_l, next) : nullptr, stats,
+                  [&](uint32_t h, float m, float l) { put[h] = float2{m, l}; });
+        if (next < 0) break;
+        cur = next;
       }
-      bad |= codec != CF_KV_CODEC_INT8 || dim != D;
-      // tokens of a page are visible from its first on
-      const uint32_t page_end = 64 * g + 16 * (n >> 2) + min(tc, 16u);
-      const uint32_t first = 64 * g + 4 * n, end = min(page_end, visible);
-      const uint32_t nvis = end > first ? min(end - first, 4u) : 0u;
-      const bool page_vis = tc > 0 && 64 * g + 16 * (n >> 2) < visible;
-      const float ks0 = ks, vs0 = vs;
-      if (next >= 0) load_k(blob_next);
-      // ---- online softmax
-      float mx[4], p[4][4], sum[4];
-      bool moved = false;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float f = unit[r] * ks0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i][r] = static_cast<uint32_t>(i) < nvis ? sc[i][r] * f : -INFINITY;
-        mx[r] = fmaxf(fmaxf(p[0][r], p[1][r]), fmaxf(p[2][r], p[3][r]));
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        mx[r] = cfd::row16_max(mx[r]);
-        moved |= mx[r] > m_run[r];
-      }
-      // units of the P.V sums: the exponent of the group's largest V scale among its visible pages, less 15, so that
-      // weights p vs lie in [0, 2^15) and those down to 2^-29 of that are normal f16 numbers. Sums move to a larger unit
-      // at once and to a smaller one when 2^8 below (a factor of a power of two; clamped so that it cannot overflow).
-      constexpr int kNone = -(1 << 24);
-      const int ep = page_vis ? __builtin_amdgcn_frexp_expf(vs0) - 15 : kNone;
-      const int eb = max(max(__builtin_amdgcn_readlane(ep, 0), __builtin_amdgcn_readlane(ep, 4)),
-                         max(__builtin_amdgcn_readlane(ep, 8), __builtin_amdgcn_readlane(ep, 12)));
-      int e_new = e_run;
-      if (eb != kNone && (eb > e_run || eb < e_run - 8)) e_new = max(eb, e_run - 60);
-      if (__builtin_amdgcn_ballot_w64(moved) || e_new != e_run) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float mn = fmaxf(m_run[r], mx[r]);
-          const float al = m_run[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[r] - mn);
-          m_run[r] = mn;
-          l_run[r] *= al;
-          const float sc2 = ldexpf(al, max(e_run - e_new, -200));  // 0 before the first visible token
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) acc[i][r] *= sc2;
-        }
-        e_run = e_new;
-      }
-      const float vsn = page_vis ? ldexpf(vs0, -e_run) : 0.0f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float m = m_run[r] == -INFINITY ? 0.0f : m_run[r];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i][r] = __builtin_amdgcn_exp2f(p[i][r] - m);  // exp2(-inf) = 0
-        sum[r] = (p[0][r] + p[1][r]) + (p[2][r] + p[3][r]);
-        l_run[r] += sum[r];
-      }
-      if (a.s.weights_out) {
-        const uint32_t slot = c0 + static_cast<uint32_t>(cur) * W;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float t = cfd::row16_sum(sum[r]);
-          if (n == r && static_cast<uint32_t>(4 * b + r) < gqa) put_stat(slot, 4 * b + r, m_run[r], t);
-        }
-      }
-      if (static_cast<uint32_t>(4 * b) < gqa) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          _Float16 h0, l0, h1, l1, h2, l2, h3, l3;
-          cfd::split2_mul_f16(p[0][r], p[1][r], vsn, h0, l0, h1, l1);
-          cfd::split2_mul_f16(p[2][r], p[3][r], vsn, h2, l2, h3, l3);
-          *reinterpret_cast<half4_t *>(&sh.p[wave][0][4 * b + r][4 * n]) = half4_t{h0, h1, h2, h3};
-          *reinterpret_cast<half4_t *>(&sh.p[wave][1][4 * b + r][4 * n]) = half4_t{l0, l1, l2, l3};
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      // ---- P.V: k-values of lane group b = tokens 8 tp .. 8 tp + 7 of page b
-#pragma unroll
-      for (int tp = 0; tp < 2; ++tp) {
-        const half8_t ph = *reinterpret_cast<const half8_t *>(&sh.p[wave][0][n][16 * b + 8 * tp]);
-        const half8_t pl = *reinterpret_cast<const half8_t *>(&sh.p[wave][1][n][16 * b + 8 * tp]);
-#pragma unroll
-        for (int i0 = 0; i0 < kTiles; i0 += 4) {
-          half8_t v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = signed_half8(vw[2 * tp * kTiles + i0 + i], vw[(2 * tp + 1) * kTiles + i0 + i]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, v[i], acc[i0 + i], 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, v[i], acc[i0 + i], 0, 0, 0);
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      if (next < 0) break;
-      load_v(blob_next);
-      cur = next;
-      blob = blob_next;
     }
+    if (!ROW && stats) write_stats(a.stats + row * a.slots * gqa, lds, mine, min(step, w1 - c0), gqa);
   }
-
+  st.bad |= bad;
+  st.close();
   // ---- join the wavefronts
-#pragma unroll
-  for (int r = 0; r < 4; ++r) l_run[r] = cfd::row16_sum(l_run[r]);
-  const bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
   if (n == 0) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {  // a NaN score leaves the maximum as it was and makes the sum a NaN
-      s_m[wave][4 * b + r] = broken || l_run[r] != l_run[r] ? __builtin_nanf("") : m_run[r];
-      s_l[wave][4 * b + r] = l_run[r];
+    for (int r = 0; r < 4; ++r) {
+      s_m[wave][4 * b + r] = st.m[r];
+      s_l[wave][4 * b + r] = st.l[r];
     }
   }
-  __syncthreads();  // (and the weight tiles are dead)
+  __syncthreads();  // (and the wavefronts' areas are dead)
   if (static_cast<uint32_t>(4 * b) < gqa) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) sh.red[wave][4 * b + r][16 * i + n] = ldexpf(acc[i][r], max(e_run, -200));
+      for (int i = 0; i < D / 16; ++i) sh.red[wave][4 * b + r][16 * i + n] = ldexpf(st.acc[i][r], max(st.e, -200));
   }
   __syncthreads();
   const size_t at = (row * a.splits + split) * gqa;
@@ -424,13 +521,151 @@ __global__ __launch_bounds__(64 * W, 2) void selected_kernel(SelArgs a) {
   }
 }
 
+// Stretches of `total` slots over nwaves wavefronts: the first total % nwaves of them one slot longer.
+struct Stretch {
+  uint32_t q, r;
+  __device__ Stretch(uint32_t total, uint32_t nwaves) : q(total / nwaves), r(total % nwaves) {}
+  __device__ uint32_t begin(uint32_t j) const { return j * q + min(j, r); }
+  __device__ uint32_t owner(uint32_t x) const { return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q; }
+};
+
+// kSpan. A wavefront's stretch touches consecutive rows; it leaves one state for each of them, number wavefront + row in
+// the laid-out order (head * seq_count + sequence), which no other wavefront has, and a row's states lie side by side.
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
+  constexpr int T = 64 * kWaves;
+  __shared__ WaveLds s_wave[kWaves];
+  __shared__ uint32_t s_pre[kSpanSeqs + 1], s_vis[kSpanSeqs], s_tot[kWaves];
+  const uint32_t tid = threadIdx.x, S = a.d.seq_count, lane = tid & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t gqa = a.d.query_head_count / a.d.kv_head_count;
+  uint32_t base = 0;
+  for (uint32_t c = 0; c < S; c += T) {
+    const uint32_t s = c + tid;
+    uint32_t n = 0, total;
+    if (s < S) {
+      const uint32_t vis = visible_tokens(a.d.seq_tokens[s], a.d.query_pos[s], a.d.max_groups);
+      n = row_slots(a, (vis + 63) / 64);
+      s_vis[s] = vis;
+    }
+    uint32_t before = base + cfsel::wave_prefix(n, total);
+    if (c) __syncthreads();
+    if (lane == 0) s_tot[wave] = total;
+    __syncthreads();
+    for (uint32_t w = 0; w < kWaves; ++w) {
+      if (w < wave) before += s_tot[w];
+      base += s_tot[w];
+    }
+    if (s < S) s_pre[s] = before;
+  }
+  if (tid == 0) s_pre[S] = base;
+  __syncthreads();
+  const uint32_t per_head = base;
+  if (blockIdx.x == 0)
+    for (uint32_t i = tid; i <= S; i += T) a.pre[i] = s_pre[i];
+  const uint32_t me = blockIdx.x * kWaves + wave;
+  if (me >= a.nwaves) return;
+  const Stretch part(per_head * a.d.kv_head_count, a.nwaves);
+  const uint32_t x0 = part.begin(me), x1 = part.begin(me + 1), step = look_slots(gqa);
+  const bool stats = a.s.weights_out != nullptr;
+  if (x0 >= x1) return;
+  WaveLds &lds = s_wave[wave];
+
+  // Lane i looks up slot x + i of the stretch: its row, group and blob.
+  struct Look {
+    uint32_t row, g, off, dest, vis;  // dest: the place of the slot's statistics
+    bool here, bad;
+  };
+  auto look = [&](uint32_t x) {
+    Look k{};
+    const uint32_t y = x + lane;
+    k.g = 0xFFFFFFFFu;
+    k.here = false;
+    k.bad = false;
+    if (y < x1 && lane < step) {
+      const uint32_t head = y / per_head, z = y - head * per_head;
+      uint32_t lo = 0, hi = S;  // the last sequence that begins at or before z: one that holds it
+      while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (s_pre[mid] <= z) lo = mid;
+        else hi = mid;
+      }
+      k.row = head * S + lo;
+      const uint32_t slot = z - s_pre[lo];
+      k.vis = s_vis[lo];
+      const size_t r = static_cast<size_t>(lo) * a.d.kv_head_count + head;
+      k.dest = static_cast<uint32_t>(r) * a.slots + slot;
+      k.g = listed_group(a, a.s.units ? a.s.units + r * a.s.max_units : nullptr, slot, k.bad);
+      k.here = k.g < (k.vis + 63) / 64;
+      if (k.here) k.off = a.d.group_offsets[r * a.d.max_groups + k.g];
+      else if (stats)
+        for (uint32_t h = 0; h < gqa; ++h) lds.stat[lane * gqa + h] = float2{-INFINITY, 0.0f};
+    }
+    return k;
+  };
+  auto lane_of = [](uint32_t x, int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(x, i)); };
+
+  RowState<D> st;
+  st.reset();
+  Blob<D> w;
+  Look k{};
+  uint32_t x = x0 - step, row = 0, q_row = 0xFFFFFFFFu;
+  uint64_t todo = 0;
+  bool first = true, in_flight = false;
+  auto row_broken = [&] { return __builtin_amdgcn_ballot_w64(k.bad && k.row == row) != 0; };
+  for (;;) {
+    const bool group = todo != 0;
+    const int cur = group ? __builtin_ctzll(todo) : static_cast<int>(min(step, x1 - x) - 1);
+    const bool done = !group && !first && x + step >= x1;
+    if (!group && !first && stats) write_stats(a.stats, lds, k.dest, min(step, x1 - x), gqa);
+    // rows up to the one at hand are closed; those without a group in this stretch leave an empty state
+    const uint32_t r = lane_of(k.row, cur) + (done ? 1u : 0u);
+    if (!first)
+      for (; row != r; ++row) {
+        st.bad |= row_broken();
+        st.close();
+        const size_t state = static_cast<size_t>(me) + row;
+        st.store(a.sums + state * gqa * D, a.states + state * gqa, gqa);
+        st.reset();
+      }
+    if (done) break;
+    if (!group) {  // the next slots
+      if (!first) st.bad |= row_broken();
+      x += step;
+      k = look(x);
+      todo = __builtin_amdgcn_ballot_w64(k.here);
+      if (first) row = lane_of(k.row, 0);
+      first = false;
+      in_flight = false;
+      continue;
+    }
+    if (!in_flight) {
+      w.load_k(blob_at(a, k.off, cur));
+      w.load_v(blob_at(a, k.off, cur));
+      in_flight = true;
+    }
+    const uint32_t seq = row % S, head = row / S;
+    if (q_row != row) {
+      Query<D> q;
+      q.load(a, seq, head, gqa);
+      st.set_query(a, q, gqa);
+      q_row = row;
+    }
+    todo &= todo - 1;
+    const uint8_t *next = todo ? blob_at(a, k.off, __builtin_ctzll(todo)) : nullptr;
+    float2 *put = lds.stat + static_cast<uint32_t>(cur) * gqa;
+    st.attend(w, lane_of(k.g, cur), lane_of(k.vis, cur), gqa, lds, next, stats,
+              [&](uint32_t h, float m, float l) { put[h] = float2{m, l}; });
+  }
+}
+
 constexpr int kJoinThreads = 512;
 constexpr uint32_t kJoinGroups = 1024;  // groups whose weights one workgroup writes
 
 // Joins a row's states: grid (KV heads, sequences, query heads + parts of the weights). A workgroup z < gqa makes the
 // output of query head z; the others turn group statistics into weights, kJoinGroups groups each. Values of many states are
 // loaded at a time: the caches of other dies hold them, so that each load takes about a microsecond.
-template <int D>
+template <int D, bool SPAN>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a) {
   constexpr int kParts = kJoinThreads / D;
   constexpr uint32_t kB = 8;
@@ -439,8 +674,20 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a) {
   const uint32_t head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const uint32_t gqa = a.d.query_head_count / a.d.kv_head_count;
   const size_t row = static_cast<size_t>(seq) * a.d.kv_head_count + head;
-  const size_t state0 = row * a.splits;
-  const uint32_t states = a.splits;
+  size_t state0 = row * a.splits;
+  uint32_t states = a.splits;
+  if constexpr (SPAN) {
+    const uint32_t per_head = a.pre[a.d.seq_count], at = a.pre[seq], len = a.pre[seq + 1] - at;
+    states = 0;
+    if (len) {
+      const Stretch part(per_head * a.d.kv_head_count, a.nwaves);
+      const uint32_t x = head * per_head + at, j = part.owner(x);
+      states = part.owner(x + len - 1) - j + 1;
+      state0 = static_cast<size_t>(j) + static_cast<size_t>(head) * a.d.seq_count + seq;
+    } else {
+      state0 = 0;
+    }
+  }
   const float2 *st = a.states + state0 * gqa;
   const bool out = blockIdx.z < gqa;
   // the sums of this thread's first states, in flight while the maxima are found
@@ -449,7 +696,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a) {
   float o8[kB];
 #pragma unroll
   for (uint32_t u = 0; u < kB; ++u)
-    o8[u] = out ? sums[static_cast<size_t>(min(part + u * kParts, states - 1)) * gqa * D] : 0.0f;
+    o8[u] = out && states ? sums[static_cast<size_t>(min(part + u * kParts, states - 1)) * gqa * D] : 0.0f;
   // a wavefront per query head: its maximum and the inverse of its sum
   for (uint32_t h = out ? blockIdx.z : tid >> 6; h < (out ? blockIdx.z + 1 : gqa); h += kJoinThreads / 64) {
     float m = -INFINITY, l = 0.0f;
@@ -511,10 +758,10 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a) {
 }
 
 struct Plan {
-  bool row;
-  uint32_t slots, splits, per;
-  uint64_t sum_bytes, state_bytes, stat_bytes;
-  uint64_t bytes() const { return sum_bytes + state_bytes + stat_bytes; }
+  Mode mode;
+  uint32_t slots, splits, per, nwaves;
+  uint64_t pre_bytes, sum_bytes, state_bytes, stat_bytes;
+  uint64_t bytes() const { return pre_bytes + sum_bytes + state_bytes + stat_bytes; }
 };
 
 uint64_t round16(uint64_t x) { return (x + 15) / 16 * 16; }
@@ -525,42 +772,62 @@ Plan make_plan(const cf_kv_batched_desc *d, const cf_kv_selection *s) {
   const uint64_t rows = static_cast<uint64_t>(d->seq_count) * d->kv_head_count, all = rows * p.slots;
   const uint32_t gqa = d->query_head_count / d->kv_head_count, cus = cfd::cu_count();
   const bool fits = static_cast<uint64_t>(p.slots) * gqa <= kRowStats;  // a row's statistics in LDS
-  uint32_t splits = d->splits;
-  // One workgroup per row where its statistics fit and the rows fill the chip: a list makes them alike in length, and where
-  // there are many of them they even out. 248 rows of 64 listed groups: 47 us, against 53 to 61 as 2 to 8 splits and the
-  // second launch. Rows of unlike length that are not many (no list) would wait for the longest: those are split, which
-  // costs 256 rows of 512 groups each 349 us instead of 321.
-  if (splits == 0 && fits && ((s->units && 4 * rows >= 3 * cus) || rows >= 8 * cus)) splits = 1;
-  if (splits == 0) {
-    // one resident round of wavefronts (two workgroups of four per CU) where there are few slots, at most 16 slots a
-    // wavefront where there are many
-    const uint64_t per_wave = std::min<uint64_t>(16, std::max<uint64_t>(1, all / (8ull * cus)));
-    splits = static_cast<uint32_t>((p.slots + per_wave * kWaves - 1) / (per_wave * kWaves));
+  uint64_t states = 0;
+  // us of a call with weights, 8 KV heads, head_dim 128, 4 query heads per KV head unless said, as kSpan / kRow / kSplit:
+  //   32 x 64 of up to 512 groups (list)     61.1 /  46.2 /  53.1      32 x 512 groups            341.3 / 320.7 / 350.9
+  //   1 x 32 groups (list)                   13.0 /  19.1 /  11.9      32 x 8..512 groups         182.0 / 234.4 / 210.9
+  //   16 x 64 groups, 8 query heads          41.2 /  36.0 /  36.8      1 x 512 groups              29.1 / 194.5 /  21.4
+  //   64 x 32 groups                         65.2 /  53.0 /  56.4      1 x 2048 groups             60.3 / 749.8 /  52.9
+  //   64 x 16..125 groups of hd 64           80.2 /  75.1 /  96.1      4 x 2048 groups            164.4 / 760.2 / 171.7
+  //   128 x 32 of 128 groups (list)         111.8 / 105.7 / 106.7      256 x 8..32 groups         158.1 / 147.1 / 146.4
+  // A row to a workgroup where a list makes the rows alike and they fill the chip once, or where they are many and even out
+  // by themselves; stretches from 16 slots a resident wavefront on, where its state is small beside them; else splits.
+  if (d->splits == 1 && fits) p.mode = kRow;
+  else if (d->splits != 0) p.mode = kSplit;
+  else if (fits && ((s->units && 4 * rows >= 3 * cus && rows <= cus) || rows >= 2 * cus)) p.mode = kRow;
+  else if (d->seq_count <= kSpanSeqs && all >= 16ull * kResident * cus && all < 1u << 31) p.mode = kSpan;
+  else p.mode = kSplit;
+  if (p.mode == kSplit) {
+    uint32_t splits = d->splits;
+    if (splits == 0) {  // one resident round of wavefronts where there are few slots, at most 16 slots each
+      const uint64_t per_wave = std::min<uint64_t>(16, std::max<uint64_t>(1, all / (static_cast<uint64_t>(kResident) * cus)));
+      splits = static_cast<uint32_t>((p.slots + per_wave * kWaves - 1) / (per_wave * kWaves));
+    }
+    splits = std::max<uint32_t>(1, std::min(splits, p.slots));
+    p.per = (p.slots + splits - 1) / splits;
+    p.splits = (p.slots + p.per - 1) / p.per;
+    states = rows * p.splits;
+  } else if (p.mode == kSpan) {
+    p.nwaves = kResident * cus;
+    p.pre_bytes = round16((d->seq_count + 1ull) * sizeof(uint32_t));
+    states = p.nwaves + rows;
+  } else {
+    p.splits = 1;
   }
-  splits = std::max<uint32_t>(1, std::min(splits, p.slots));
-  p.per = (p.slots + splits - 1) / splits;
-  p.splits = (p.slots + p.per - 1) / p.per;
-  p.row = p.splits == 1 && fits;
-  if (!p.row) {
-    p.sum_bytes = round16(rows * p.splits * gqa * d->head_dim * sizeof(float));
-    p.state_bytes = round16(rows * p.splits * gqa * sizeof(float2));
-    p.stat_bytes = s->weights_out ? all * gqa * sizeof(float2) : 0;
-  }
+  p.sum_bytes = round16(states * gqa * d->head_dim * sizeof(float));
+  p.state_bytes = round16(states * gqa * sizeof(float2));
+  p.stat_bytes = s->weights_out && p.mode != kRow ? all * gqa * sizeof(float2) : 0;
   return p;
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <int D>
-void launch(const SelArgs &a, bool row, hipStream_t s) {
+void launch(const SelArgs &a, Mode mode, hipStream_t s) {
   const uint32_t heads = a.d.kv_head_count, seqs = a.d.seq_count;
-  if (row) {
-    selected_kernel<D, kWavesRow, true><<<dim3(1, heads, seqs), 64 * kWavesRow, 0, s>>>(a);
+  if (mode == kRow) {
+    row_kernel<D, kWavesRow, true><<<dim3(1, heads, seqs), 64 * kWavesRow, 0, s>>>(a);
     return;
   }
-  selected_kernel<D, kWaves, false><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
   const uint32_t parts = a.s.weights_out ? (a.d.max_groups + kJoinGroups - 1) / kJoinGroups : 0;
-  join_kernel<D><<<dim3(heads, seqs, a.d.query_head_count / heads + parts), kJoinThreads, 0, s>>>(a);
+  const dim3 join(heads, seqs, a.d.query_head_count / heads + parts);
+  if (mode == kSpan) {
+    span_kernel<D><<<(a.nwaves + kWaves - 1) / kWaves, 64 * kWaves, 0, s>>>(a);
+    join_kernel<D, true><<<join, kJoinThreads, 0, s>>>(a);
+  } else {
+    row_kernel<D, kWaves, false><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
+    join_kernel<D, false><<<join, kJoinThreads, 0, s>>>(a);
+  }
 }
 
 }  // namespace
@@ -602,11 +869,12 @@ extern "C" cf_status cf_kv_paged_attention_selected_async(const cf_kv_batched_de
   const uint64_t need = p.bytes();
   if (need && (!d->workspace || d->workspace_bytes < need || !aligned16(d->workspace))) return CF_ERR_INVALID_ARGUMENT;
   char *ws = static_cast<char *>(d->workspace);
-  SelArgs a{*d, *s, p.slots, p.splits, p.per, reinterpret_cast<float *>(ws), reinterpret_cast<float2 *>(ws + p.sum_bytes),
-            reinterpret_cast<float2 *>(ws + p.sum_bytes + p.state_bytes)};
+  SelArgs a{*d, *s, p.slots, p.splits, p.per, p.nwaves, reinterpret_cast<uint32_t *>(ws),
+            reinterpret_cast<float *>(ws + p.pre_bytes), reinterpret_cast<float2 *>(ws + p.pre_bytes + p.sum_bytes),
+            reinterpret_cast<float2 *>(ws + p.pre_bytes + p.sum_bytes + p.state_bytes)};
   if (!s->units) a.s.unit_groups = 1;
   const hipStream_t st = cfd::as_stream(stream);
-  if (d->head_dim == 128) launch<128>(a, p.row, st);
-  else launch<64>(a, p.row, st);
+  if (d->head_dim == 128) launch<128>(a, p.mode, st);
+  else launch<64>(a, p.mode, st);
   return cfd::launch_status();
 }

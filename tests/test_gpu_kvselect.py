@@ -303,6 +303,55 @@ def test_attention_many_groups_per_wavefront(dev):
     c.check(c.lists(290, 1, 0.95), splits=(1,))
 
 
+@pytest.mark.parametrize("S, H, D, gqa, longest", [(300, 2, 128, 4, 4096), (700, 1, 64, 7, 3300), (1030, 1, 64, 2, 2600)])
+@pytest.mark.parametrize("unit", [0, 1, 2])
+def test_attention_many_ragged_sequences(dev, S, H, D, gqa, longest, unit):
+    """Lengths from nothing to long ones side by side, most rows shorter than a wavefront's stretch of the slots: stretches
+    over several rows, rows over several stretches, empty rows inside and at both ends of them (1030 sequences: too many
+    for stretches, the splits behind them)."""
+    rng = np.random.default_rng(S + unit)
+    lens = rng.integers(0, 150, S)
+    lens[rng.random(S) < 0.3] = 0
+    lens[[0, -1]] = 0
+    lens[S // 2] = longest
+    lens[S // 3] = 700
+    c = Case(dev, [int(t) for t in lens], H, gqa, D, S)
+    w = rng.random((S, H, c.M)).astype(np.float32)
+    if unit == 0:
+        c.check(weights=w)
+        c.check(want=False)
+    else:
+        c.check(c.lists(-(-c.M // unit), unit, 0.6), unit, weights=w)
+
+
+def test_attention_broken_lists_among_ragged_sequences(dev):
+    # entries that do not ascend, in rows that lie in one stretch, across stretches, without a visible unit listed before them
+    rng = np.random.default_rng(3)
+    S, M = 600, 64
+    lens = [int(x) for x in rng.integers(1, 300, S)]
+    lens[100], lens[101], lens[400] = 64 * M, 64 * M, 64 * M
+    c = Case(dev, lens, 1, 4, 64, 71)
+    lists = np.full((S, 1, M), R.NO_UNIT, np.uint32)
+    for s in range(S):
+        n = -(-lens[s] // 64)
+        lists[s, 0, :n] = np.arange(n)
+    bad = [100, 400, 7, 250]
+    lists[100, 0, 63] = 10
+    lists[400, 0, 30] = 60
+    for s in (7, 250):
+        lens_s = -(-lens[s] // 64)
+        lists[s, 0, :2] = [1, 0] if lens_s > 1 else [0, 0]
+        if lens_s < 2:
+            bad.remove(s)  # one unit can be listed: its entry is all that is read
+    out, _ = c.run(lists)
+    ok = np.ones(S, bool)
+    ok[bad] = False
+    assert np.isnan(out[bad]).all() and np.isfinite(out[ok]).all()
+    ref = R.attend_ref(c.q, c.k, c.v, c.lens, c.pos, c.gqa, c.scale, lists, 1, c.M)
+    tol = R.tolerance(ref[3], c.D)
+    assert (np.abs(out - ref[0]) <= tol[..., None] * ref[2] + 2.0 ** -23 * np.abs(ref[0]) + ref[4])[ok].all()
+
+
 def test_attention_weights_forms(dev):
     import torch
     from chromofold_amd import kvselect as ks
