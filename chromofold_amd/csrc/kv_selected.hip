@@ -1,6 +1,7 @@
-// kv_selected.hip — attention over selected groups of an INT8 pool, with the groups' attention weight
+// kv_selected.hip — attention over selected groups of a pool, with the groups' attention weight
 // (chromofold/kv_select.h, cf_kv_paged_attention_selected_async).
 //
+// The kernels for INT8 pools; the one for RANS_HYBRID pools stands at the end and shares the cuts, joins and weights.
 // Per (sequence, KV head), over the tokens t of the listed groups, query heads h of the KV head:
 //   s_ht = scale q_h . (ks_page (sym - 128)_t),  p = softmax_t(s),  o_h = sum_t p_ht vs_page (sym - 128)_t,
 //   weights_out[g] = decay weights_in[g] + sum_h sum_{t in g} p_ht.
@@ -27,6 +28,7 @@
 
 #include "cf_device.hpp"
 #include "chromofold/kv_select.h"
+#include "kv_group_body.hpp"
 #include "kv_topk.hpp"
 
 namespace {
@@ -54,7 +56,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 //           and a wavefront's loads run on from one row into the next.
 //   kRow    a workgroup per row, which finishes it: no second launch
 //   kSplit  `splits` workgroups per row, `per` slots each: a row's result depends on its own sequence alone
-enum Mode { kSpan, kRow, kSplit };
+//   kCoded  kSplit for RANS_HYBRID pools, `per` a multiple of the groups of a unit
+enum Mode { kSpan, kRow, kSplit, kCoded };
 
 struct SelArgs {
   cf_kv_batched_desc d;
@@ -381,14 +384,14 @@ __device__ __forceinline__ const uint8_t *blob_at(const SelArgs &a, uint32_t off
 }
 
 // Statistics of `count` slots looked up together from the wavefront's LDS to memory; `dest`: the place of this lane's slot.
-__device__ __forceinline__ void write_stats(float2 *__restrict__ to, const WaveLds &lds, uint32_t dest, uint32_t count, uint32_t gqa) {
+__device__ __forceinline__ void write_stats(float2 *__restrict__ to, const float2 *stat, uint32_t dest, uint32_t count, uint32_t gqa) {
   const uint32_t lane = threadIdx.x & 63;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
   for (uint32_t e0 = 0; e0 < count * gqa; e0 += 64) {
     const uint32_t e = e0 + lane, i = min(e / gqa, 63u);
     const size_t at = __shfl(dest, static_cast<int>(i));
-    if (e < count * gqa) to[at * gqa + (e - i * gqa)] = lds.stat[e];
+    if (e < count * gqa) to[at * gqa + (e - i * gqa)] = stat[e];
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -462,7 +465,7 @@ __global__ __launch_bounds__(64 * W, 2) void row_kernel(SelArgs a) {
         cur = next;
       }
     }
-    if (!ROW && stats) write_stats(a.stats + row * a.slots * gqa, lds, mine, min(step, w1 - c0), gqa);
+    if (!ROW && stats) write_stats(a.stats + row * a.slots * gqa, lds.stat, mine, min(step, w1 - c0), gqa);
   }
   st.bad |= bad;
   st.close();
@@ -617,7 +620,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
     const bool group = todo != 0;
     const int cur = group ? __builtin_ctzll(todo) : static_cast<int>(min(step, x1 - x) - 1);
     const bool done = !group && !first && x + step >= x1;
-    if (!group && !first && stats) write_stats(a.stats, lds, k.dest, min(step, x1 - x), gqa);
+    if (!group && !first && stats) write_stats(a.stats, lds.stat, k.dest, min(step, x1 - x), gqa);
     // rows up to the one at hand are closed; those without a group in this stretch leave an empty state
     const uint32_t r = lane_of(k.row, cur) + (done ? 1u : 0u);
     if (!first)
@@ -656,6 +659,262 @@ __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
     float2 *put = lds.stat + static_cast<uint32_t>(cur) * gqa;
     st.attend(w, lane_of(k.g, cur), lane_of(k.vis, cur), gqa, lds, next, stats,
               [&](uint32_t h, float m, float l) { put[h] = float2{m, l}; });
+  }
+}
+
+// ---- RANS_HYBRID pools: the batched decode's group body (kv_group_body.hpp; at most 4 query heads per KV head), groups of a
+// unit decoded back to back by one wavefront, since a chain may run across them. Bound by the entropy decode, as there: the
+// tables are staged by every workgroup and the memory pipeline restarts at every row. 32 pairs of 512 groups for each of
+// 32 x 8 rows (252 MB) 68 us, all their 512 groups (2.02 GB) 477, 462 without weights (kv_batched.hip 374-396). Two wavefronts a SIMD: at three the
+// code for raw groups beside the lookups spills (75 and 478 us with 13 registers spilled, 111 and 622 with 58).
+
+// A unit's groups in this launch: the list's units, or pairs (a chain never spans more).
+__host__ __device__ inline uint32_t coded_item(const cf_kv_selection &s) { return s.units ? s.unit_groups : 2u; }
+
+template <int D>
+__global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWaves) void coded_kernel(SelArgs a) {
+  using namespace cfkv;
+  constexpr int W = kWaves, NQ = D / 4, RAW = raw_words<D>(), BUF = buf_u32<D>(), T = 64 * W;
+  __shared__ __attribute__((aligned(16))) uint2 s_tab[2][kSlots];
+  __shared__ __attribute__((aligned(16))) _Float16 s_p[W][2][4][kGqa][16];
+  __shared__ uint32_t s_buf[W][BUF];  // per wavefront: staged words; query staging and the joined states alias it
+  static_assert(2 * kGqa * D * 2 <= W * BUF * 4, "query staging must fit the word buffers");
+  const int lane = threadIdx.x & 63, G = lane >> 4, t = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t head = blockIdx.y, seq = blockIdx.z;
+  const uint32_t gqa = a.d.query_head_count / a.d.kv_head_count;
+  const size_t row = static_cast<size_t>(seq) * a.d.kv_head_count + head;
+  const uint32_t split = (blockIdx.x + static_cast<uint32_t>(row % a.splits)) % a.splits;  // (see row_kernel)
+  const uint32_t *list = a.s.units ? a.s.units + row * a.s.max_units : nullptr;
+  const uint32_t *grow = a.d.group_offsets + row * a.d.max_groups;
+  const uint32_t visible = visible_tokens(a.d.seq_tokens[seq], a.d.query_pos[seq], a.d.max_groups);
+  const uint32_t ngroups = (visible + 63) / 64, nslots = row_slots(a, ngroups), item = coded_item(a.s);
+  const uint32_t s0 = min(split * a.per, nslots), s1 = min(nslots, s0 + a.per);
+
+  // ---- tables and queries, as kv_batched_kernel stages them
+  {
+    const uint4 *tk = reinterpret_cast<const uint4 *>(a.d.tables + static_cast<size_t>(2 * head) * CF_KV_RANS_TABLE_BYTES);
+    constexpr int kIt = static_cast<int>(kSlots / T);
+    static_assert(kSlots % T == 0, "two table entries a thread and step");
+    uint4 e[kIt];
+#pragma unroll
+    for (int k = 0; k < kIt; ++k) e[k] = tk[threadIdx.x + k * T];
+#pragma unroll
+    for (int k = 0; k < kIt; ++k) {
+      const uint32_t j = 2 * (threadIdx.x + k * T);
+      *reinterpret_cast<uint4 *>(&s_tab[j / kSlots][j % kSlots]) =
+          uint4{(e[k].x & 2047u) | (((e[k].x >> 11) & 2047u) << 16), e[k].y,
+                (e[k].z & 2047u) | (((e[k].z >> 11) & 2047u) << 16), e[k].w};
+    }
+  }
+  _Float16(*s_q)[kGqa][D] = reinterpret_cast<_Float16(*)[kGqa][D]>(&s_buf[0][0]);
+  for (int i = threadIdx.x; i < kGqa * D; i += T) {
+    const int h = i / D, dd = i % D;
+    const float q = static_cast<uint32_t>(h) < gqa
+                        ? a.d.queries[(static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + h) * D + dd]
+                        : 0.0f;
+    cfd::split_mul_f16(q, a.d.softmax_scale, s_q[0][h][dd], s_q[1][h][dd]);
+  }
+  __syncthreads();
+  constexpr int NC = NQ / 16 > 0 ? NQ / 16 : 1;
+  cfkv::half4_t qhi[NC], qlo[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int qd = 16 * c + (lane >> 2);
+    qhi[c] = (4 * qd < D) ? *reinterpret_cast<const cfkv::half4_t *>(&s_q[0][lane & 3][4 * qd]) : cfkv::half4_t{0, 0, 0, 0};
+    qlo[c] = (4 * qd < D) ? *reinterpret_cast<const cfkv::half4_t *>(&s_q[1][lane & 3][4 * qd]) : cfkv::half4_t{0, 0, 0, 0};
+  }
+  float qsum[kGqa];
+  {
+    float part = 0.0f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+      part += static_cast<float>(s_q[0][G][t * (D / 16) + k]) + static_cast<float>(s_q[1][G][t * (D / 16) + k]);
+    part = cfd::row16_sum(part);
+#pragma unroll
+    for (int h = 0; h < kGqa; ++h) qsum[h] = __shfl(part, 16 * h);
+  }
+  __syncthreads();  // s_q is dead from here on
+
+  float m_run[kGqa], l_run[kGqa];
+  int e_run = -(1 << 20);
+  cfkv::float4_t acc_v[D / 16];
+#pragma unroll
+  for (int h = 0; h < kGqa; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) acc_v[i] = cfkv::float4_t{0, 0, 0, 0};
+
+  uint32_t *buf = s_buf[wave];
+  const bool stats = a.s.weights_out != nullptr;
+  bool bad = false;  // a list that does not ascend, or a group that continues a chain its unit does not begin
+  // blocks of whole units for the wavefronts; slots are looked up 64 at a time, one a lane
+  const uint32_t items = (s1 - s0 + item - 1) / item, pw = (items + W - 1) / W * item;
+  const uint32_t w0 = min(s1, s0 + wave * pw), w1 = min(s1, w0 + pw);
+  for (uint32_t c0 = w0; c0 < w1; c0 += 64) {
+    const uint32_t mine = c0 + lane;
+    uint32_t g_l = 0xFFFFFFFFu, off_l = 0;
+    if (mine < w1) {
+      g_l = listed_group(a, list, mine, bad);
+      if (g_l < ngroups) off_l = grow[g_l];
+    }
+    const bool here = g_l < ngroups;
+    uint64_t todo = __builtin_amdgcn_ballot_w64(here);
+    float2 stat[kGqa];  // of this lane's slot
+#pragma unroll
+    for (int h = 0; h < kGqa; ++h) stat[h] = float2{-INFINITY, 0.0f};
+    if (todo) {
+      // The memory pipeline is kv_batched_kernel's: the next group's header and chain states at the start of a group, its word
+      // streams into the wavefront's LDS after the decode, its first raw words as the last of this group's are used up.
+      uint32_t h_cnt = 0, h_chain = 0, h_tc = 0, h_codec = 0, h_st[2] = {0, 0};
+      float h_ks = 0.f, h_vs = 0.f;
+      auto load_header = [&](const uint8_t *p) {
+        h_st[0] = reinterpret_cast<const uint32_t *>(p + cfkv::kHdr)[lane];
+        h_st[1] = reinterpret_cast<const uint32_t *>(p + cfkv::kHdr)[64 + lane];
+        h_cnt = *reinterpret_cast<const uint32_t *>(p + 4);
+        h_chain = *reinterpret_cast<const uint16_t *>(p + 8);
+        h_tc = reinterpret_cast<const uint16_t *>(p + 12)[G];
+        h_ks = reinterpret_cast<const float *>(p + 32)[G];
+        h_vs = reinterpret_cast<const float *>(p + 48)[G];
+        h_codec = *reinterpret_cast<const uint32_t *>(p);
+      };
+      auto raw_of = [&](const uint8_t *p, uint32_t chain) {
+        return reinterpret_cast<const uint32_t *>(p + cfkv::kHdr + (chain ? kStateBytes : 0));
+      };
+      constexpr int kStage16 = ((kCapWords * 2) + 1023) / 1024;
+      auto stage_words = [&](const uint8_t *p, uint32_t chain, uint32_t cnt) {
+        const uint32_t nbytes = ((min((cnt & 0xFFFFu) + (cnt >> 16), kCapWords) * 2u) + 15u) & ~15u;
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(raw_of(p, chain) + 2 * RAW) + 16u * lane;
+#pragma unroll
+        for (int k = 0; k < kStage16; ++k)
+          if (1024u * k + 16u * lane < nbytes)
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t *>(src + 1024 * k),
+                                             (__attribute__((address_space(3))) void *)(buf + 256 * k), 16, 0, 0);
+      };
+      int cur = __builtin_ctzll(todo);
+      const uint8_t *blob = blob_at(a, off_l, cur);
+      load_header(blob);
+      uint32_t pre[14];
+#pragma unroll
+      for (int w = 0; w < 14; ++w) pre[w] = 0;
+      if (h_codec == CF_KV_CODEC_RANS_HYBRID) {
+        const uint32_t *lw = raw_of(blob, h_chain);
+#pragma unroll
+        for (int w = 0; w < 7; ++w) {
+          pre[w] = lw[w * 64 + lane];
+          pre[7 + w] = lw[RAW + w * 64 + lane];
+        }
+        stage_words(blob, h_chain, h_cnt);
+      }
+      uint32_t st[2] = {0, 0}, prev = 0xFFFFFFFFu;
+      for (;;) {
+        const uint32_t gi = static_cast<uint32_t>(__builtin_amdgcn_readlane(g_l, cur));
+        const uint32_t cnt = h_cnt, chain = h_chain, tcG = h_tc, gcodec = h_codec;
+        const float ks = h_ks, vs = h_vs;
+        const uint8_t *here_blob = blob;
+        const bool tok_ok = static_cast<uint32_t>(t) < tcG && 64 * gi + 16 * G + t < visible;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this group's words have landed
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (gcodec == CF_KV_CODEC_RANS_HYBRID) {
+          if (chain) {
+            st[0] = h_st[0];
+            st[1] = h_st[1];
+          } else {
+            bad |= prev + 1 != gi || (c0 + static_cast<uint32_t>(cur)) % item == 0;
+          }
+        }
+        todo &= todo - 1;
+        const int next = todo ? __builtin_ctzll(todo) : -1;
+        if (next >= 0) {
+          blob = blob_at(a, off_l, next);
+          load_header(blob);
+        }
+        const bool next_rans = next >= 0 && h_codec == CF_KV_CODEC_RANS_HYBRID;
+        const uint32_t *nlw = next_rans ? raw_of(blob, h_chain) : nullptr;
+        auto stage_next = [&]() {
+          if (next_rans) stage_words(blob, h_chain, h_cnt);
+        };
+        float p[kGqa];
+        if (gcodec == CF_KV_CODEC_RANS_HYBRID)
+          group_body<D, CF_KV_CODEC_RANS_HYBRID, 0>(stage_next, pre, nlw, st, raw_of(here_blob, chain),
+                                                    reinterpret_cast<const uint16_t *>(buf), cnt, s_tab, qhi, qlo, qsum, s_p[wave],
+                                                    static_cast<uint32_t *>(nullptr), lane, tok_ok, ks, vs, e_run, m_run, l_run,
+                                                    acc_v, static_cast<uint32_t *>(nullptr), false, p);
+        else
+          group_body<D, CF_KV_CODEC_INT8, 0, const uint16_t *>(
+              stage_next, pre, nlw, st, reinterpret_cast<const uint32_t *>(here_blob + cfkv::kHdr),
+              static_cast<const uint16_t *>(nullptr), 0, s_tab, qhi, qlo, qsum, s_p[wave], static_cast<uint32_t *>(nullptr), lane,
+              tok_ok, ks, vs, e_run, m_run, l_run, acc_v, static_cast<uint32_t *>(nullptr), false, p);
+        if (stats) {
+#pragma unroll
+          for (int h = 0; h < kGqa; ++h) {
+            const float sum = cfd::rows4_sum(cfd::row16_sum(p[h]));
+            if (lane == cur) stat[h] = float2{m_run[h] * kLog2e, sum};
+          }
+        }
+        prev = gi;
+        if (next < 0) break;
+        cur = next;
+      }
+    }
+    if (stats && mine < w1) {
+#pragma unroll
+      for (int h = 0; h < kGqa; ++h)
+        if (static_cast<uint32_t>(h) < gqa) a.stats[(row * a.slots + mine) * gqa + h] = stat[h];
+    }
+  }
+
+  // ---- reduce the wavefront and join the workgroup, as kv_batched_kernel does
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int h = 0; h < kGqa; ++h) {
+      float v = G < 2 ? ldexpf(acc_v[i][h], e_run) : 0.0f;
+      v += __shfl_xor(v, 16);
+      v += __shfl_xor(v, 32);
+      acc_v[i][h] = v;
+    }
+#pragma unroll
+  for (int h = 0; h < kGqa; ++h) l_run[h] = cfd::rows4_sum(cfd::row16_sum(l_run[h]));
+  const bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
+  float *red = reinterpret_cast<float *>(buf);
+  if (lane < 16) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int h = 0; h < kGqa; ++h) red[h * (D + 2) + t + 16 * i] = acc_v[i][h];
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int h = 0; h < kGqa; ++h) {
+      red[h * (D + 2) + D] = broken || l_run[h] != l_run[h] ? __builtin_nanf("") : m_run[h];
+      red[h * (D + 2) + D + 1] = l_run[h];
+    }
+  }
+  __syncthreads();
+  const size_t at = (row * a.splits + split) * gqa;
+  for (uint32_t i = threadIdx.x; i < gqa * D; i += T) {
+    const uint32_t h = i / D, dd = i % D;
+    float m = -INFINITY, l = 0.0f, o = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float mw = reinterpret_cast<const float *>(s_buf[w])[h * (D + 2) + D];
+      nan |= mw != mw;
+      m = fmaxf(m, mw);
+    }
+    if (m != -INFINITY)
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float *rw = reinterpret_cast<const float *>(s_buf[w]) + h * (D + 2);
+        if (rw[D] == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f((rw[D] - m) * kLog2e);
+        l += rw[D + 1] * f;
+        o += rw[dd] * f;
+      }
+    a.sums[at * D + i] = o;
+    if (dd == 0) a.states[at + h] = float2{nan ? __builtin_nanf("") : m * kLog2e, l};
   }
 }
 
@@ -782,19 +1041,22 @@ Plan make_plan(const cf_kv_batched_desc *d, const cf_kv_selection *s) {
   //   128 x 32 of 128 groups (list)         111.8 / 105.7 / 106.7      256 x 8..32 groups         158.1 / 147.1 / 146.4
   // A row to a workgroup where a list makes the rows alike and they fill the chip once, or where they are many and even out
   // by themselves; stretches from 16 slots a resident wavefront on, where its state is small beside them; else splits.
-  if (d->splits == 1 && fits) p.mode = kRow;
+  if (d->codec == CF_KV_CODEC_RANS_HYBRID) p.mode = kCoded;
+  else if (d->splits == 1 && fits) p.mode = kRow;
   else if (d->splits != 0) p.mode = kSplit;
   else if (fits && ((s->units && 4 * rows >= 3 * cus && rows <= cus) || rows >= 2 * cus)) p.mode = kRow;
   else if (d->seq_count <= kSpanSeqs && all >= 16ull * kResident * cus && all < 1u << 31) p.mode = kSpan;
   else p.mode = kSplit;
-  if (p.mode == kSplit) {
+  if (p.mode == kSplit || p.mode == kCoded) {
+    const uint32_t item = p.mode == kCoded ? coded_item(*s) : 1, items = (p.slots + item - 1) / item;
+    const uint64_t resident = static_cast<uint64_t>(kResident) * cus;
     uint32_t splits = d->splits;
     if (splits == 0) {  // one resident round of wavefronts where there are few slots, at most 16 slots each
-      const uint64_t per_wave = std::min<uint64_t>(16, std::max<uint64_t>(1, all / (static_cast<uint64_t>(kResident) * cus)));
-      splits = static_cast<uint32_t>((p.slots + per_wave * kWaves - 1) / (per_wave * kWaves));
+      const uint64_t per_wave = std::min<uint64_t>(16 / item, std::max<uint64_t>(1, rows * items / resident));
+      splits = static_cast<uint32_t>((items + per_wave * kWaves - 1) / (per_wave * kWaves));
     }
-    splits = std::max<uint32_t>(1, std::min(splits, p.slots));
-    p.per = (p.slots + splits - 1) / splits;
+    splits = std::max<uint32_t>(1, std::min(splits, items));
+    p.per = (items + splits - 1) / splits * item;
     p.splits = (p.slots + p.per - 1) / p.per;
     states = rows * p.splits;
   } else if (p.mode == kSpan) {
@@ -825,7 +1087,8 @@ void launch(const SelArgs &a, Mode mode, hipStream_t s) {
     span_kernel<D><<<(a.nwaves + kWaves - 1) / kWaves, 64 * kWaves, 0, s>>>(a);
     join_kernel<D, true><<<join, kJoinThreads, 0, s>>>(a);
   } else {
-    row_kernel<D, kWaves, false><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
+    if (mode == kCoded) coded_kernel<D><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
+    else row_kernel<D, kWaves, false><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
     join_kernel<D, false><<<join, kJoinThreads, 0, s>>>(a);
   }
 }
@@ -846,7 +1109,6 @@ extern "C" cf_status cf_kv_validate_selection(const cf_kv_batched_desc *d, const
     const cf_status w = cf_kv_validate_batched_desc(&fewer);
     if (w != CF_OK) return w;
   }
-  if (d->codec != CF_KV_CODEC_INT8) return CF_ERR_UNSUPPORTED;
   if (d->max_groups == 0) return CF_ERR_INVALID_ARGUMENT;
   if (d->max_groups >= 1u << 26) return CF_ERR_UNSUPPORTED;
   if (s->units) {

@@ -213,16 +213,17 @@ def test_select_long(dev, M, unit, S):
 class Case:
     """An INT8 (or rANS) cache of given lengths, its dequantised K and V in 64 bits, queries and positions."""
 
-    def __init__(self, dev, lens, H, gqa, D, seed, pos=None, codec=1, chained=True, **how):
+    def __init__(self, dev, lens, H, gqa, D, seed, pos=None, codec=1, raw_groups=None, **how):
         from chromofold_amd import kv
         self.dev, self.lens, self.H, self.gqa, self.D = dev, lens, H, gqa, D
         data = make_seqs([max(t, 1) for t in lens], H, D, seed, **how)
         tables = None
         if codec == 2:
+            longest = int(np.argmax(lens))
             tables = np.concatenate([kv.build_table(x[h][: x.shape[1] // 16 * 16].reshape(-1, 16, D)[:32]) for h in range(H)
-                                     for x in data[0]])
+                                     for x in data[longest]])
         self.kvb = kv.build_batched(codec, lambda s: data[s], len(lens), H, np.array([max(t, 1) for t in lens]), D, tables, dev,
-                                    keep_host=True)
+                                    keep_host=True, raw_groups=raw_groups)
         self.kvb.seq_tokens.copy_(up(dev, np.array(lens, np.uint32)))
         self.k, self.v = [], []
         for s, t in enumerate(lens):
@@ -449,6 +450,60 @@ def test_attention_pool_past_32_bits(dev):
         c.kvb.pool, c.kvb.group_offsets = small, off
         del pool
         torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------------------------- coded pools
+def coded(dev, lens, H, gqa, D, seed, chained, pos=None, raw=None, **how):
+    """A RANS_HYBRID cache sealed with chain pairs (as build_batched does) or with groups of their own."""
+    from chromofold_amd import kv
+    flags = kv.pair_flags
+    if not chained:
+        kv.pair_flags = lambda g, first_coded=0: np.zeros(np.asarray(g).size, np.uint8)
+    try:
+        return Case(dev, lens, H, gqa, D, seed, pos, codec=2, raw_groups=raw, **how)
+    finally:
+        kv.pair_flags = flags
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("gqa", [1, 3, 4])
+def test_coded_pairs(dev, D, gqa):
+    lens = [0, 1, 17, 64, 65, 130, 1000, 2100, 0]
+    pos = [0, 0, 16, 63, 20, 129, 640, 2099, 5]
+    c = coded(dev, lens, 2, gqa, D, 80 + gqa, True, pos, raw={6: 3})
+    w = c.rng.random((len(lens), 2, c.M)).astype(np.float32)
+    c.check(weights=w, splits=(0, 1, 3, 17))
+    c.check(c.lists(17, 2), 2, weights=w, splits=(0, 1, 4))
+    c.check(c.lists(5, 2), 2, want=False)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_coded_groups_of_their_own(dev, D):
+    lens = [1, 64, 200, 1500, 4200]
+    c = coded(dev, lens, 2, 4, D, 90, False)
+    c.check(weights=c.rng.random((5, 2, c.M)).astype(np.float32), splits=(0, 2))
+    for unit in (1, 2):
+        c.check(c.lists(20, unit), unit, weights=c.rng.random((5, 2, c.M)).astype(np.float32), splits=(0, 1, 5))
+
+
+def test_coded_magnitudes_and_long_lists(dev):
+    coded(dev, [700, 640, 130], 2, 4, 128, 41, True, v_mult=[[1e-2, 1e7], [1e-5, 1e3], [1.0, 1e-30]]).check(splits=(0, 1))
+    c = coded(dev, [64 * 150, 64 * 149 + 1], 1, 4, 64, 91, True)  # more than 64 slots a wavefront
+    c.check(splits=(1,), weights=c.rng.random((2, 1, c.M)).astype(np.float32))
+    c.check(c.lists(70, 2, 0.95), 2, splits=(1,))
+
+
+def test_coded_groups_that_continue_a_chain_are_not_single_units(dev):
+    c = coded(dev, [640, 640, 640], 2, 4, 128, 92, True)
+    lists = np.full((3, 2, 3), R.NO_UNIT, np.uint32)
+    lists[:, :, :2] = [0, 4]      # even groups begin their chains
+    lists[1, 0, :2] = [0, 3]      # an odd one on its own
+    lists[2, 1, :2] = [4, 5]      # a pair, but as two units
+    out, w = c.run(lists)
+    assert np.isnan(out[1, :4]).all() and np.isnan(out[2, 4:]).all()
+    assert np.isfinite(out[0]).all() and np.isfinite(out[1, 4:]).all() and np.isfinite(out[2, :4]).all()
+    out, _ = c.run(np.where(lists == R.NO_UNIT, R.NO_UNIT, [[[0, 1, 0]]]).astype(np.uint32), 2)
+    assert np.isfinite(out).all()
 
 
 # ---------------------------------------------------------------------------------------------------- eviction
