@@ -14,7 +14,7 @@ __device__ __forceinline__ uint32_t sortable(float x) {
 }
 
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kFew = 64;   // so few keys are ranked by comparing each with all
+constexpr uint32_t kFew = 96;   // so few keys are ranked by comparing each with all
 
 template <int T>
 struct TopkShared {
@@ -23,17 +23,41 @@ struct TopkShared {
   uint32_t lo, hi, bin, above, count;
 };
 
-// Sum of x over the lanes below this one (exclusive) and over the whole wavefront.
+// Lane moves inside the rows of 16 lanes and between rows by DPP, which keep an LDS round trip per step (ds_bpermute) off
+// the picks' dependency chain; lanes without a source get 0.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_all(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), CTRL, 0xf, 0xf, false));
+}
+
+// Sum of x over the lanes below this one (exclusive) and over the whole wavefront: row_shr 1, 2, 4, 8 inside the rows,
+// then row_bcast 15 (into rows 1 and 3) and 31 (into rows 2 and 3).
 __device__ __forceinline__ uint32_t wave_prefix(uint32_t x, uint32_t &total) {
-  const int lane = threadIdx.x & 63;
   uint32_t s = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t y = __shfl_up(s, o);
-    if (lane >= o) s += y;
-  }
-  total = __shfl(s, 63);
+  s += dpp_or_0<0x111>(s);
+  s += dpp_or_0<0x112>(s);
+  s += dpp_or_0<0x114>(s);
+  s += dpp_or_0<0x118>(s);
+  s += dpp_or_0<0x142, 0xa>(s);
+  s += dpp_or_0<0x143, 0xc>(s);
+  total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(s), 63));
   return s - x;
+}
+
+// Largest x of the wavefront, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max(x, dpp_all<0xb1>(x));
+  x = max(x, dpp_all<0x4e>(x));
+  x = max(x, dpp_all<0x141>(x));
+  x = max(x, dpp_all<0x140>(x));
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+  const auto h = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(static_cast<uint32_t>(h[0]), static_cast<uint32_t>(h[1]));
 }
 
 // Keys key(i) > 0, i < n; of them [0, first) and [n - last, n) are in whatever their keys; k in all are taken,
@@ -45,7 +69,7 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t x, uint32_t &total) {
 // their sign and most of their exponent, so fixed digits would send most keys to one counter), the bin where the count
 // from the top reaches what is still needed becomes the next range; at most three rounds for 32 bits, mostly one or two:
 // a round ends the search when its bin is needed whole. Up to kFew keys: each is compared with all others, one barrier
-// instead of about ten (64 units of 256 rows 8.0 -> 7.0 us; 128 units 8.5 -> 9.1).
+// instead of about ten (eviction of one of 65 units, a third of them equal, 8.1 -> 6.0 us; 128 units 7.6 -> 8.2).
 template <int T, typename Key, typename Emit, typename RoundEnd>
 __device__ __forceinline__ void take_largest(const Key &key, uint32_t n, uint32_t first, uint32_t last, uint32_t k,
                                              TopkShared<T> &sh, const Emit &emit, const RoundEnd &round_end) {
@@ -65,12 +89,18 @@ __device__ __forceinline__ void take_largest(const Key &key, uint32_t n, uint32_
       const uint32_t mine = free ? key(tid) : 0u;  // 0: below every key
       if (tid < kFew) sh.hist[tid] = mine;
       __syncthreads();
+      // before this wavefront's indices an equal key counts, behind them it does not; among them it is decided lane by lane
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < n; j += 4) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(&sh.hist[j]);
-        rank += (x.x > mine || (x.x == mine && j < tid)) + (x.y > mine || (x.y == mine && j + 1 < tid)) +
-                (x.z > mine || (x.z == mine && j + 2 < tid)) + (x.w > mine || (x.w == mine && j + 3 < tid));
-      }
+      auto count = [&](uint32_t from, uint32_t to, auto above) {
+        for (uint32_t j = from; j < min(to, n); j += 4) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(&sh.hist[j]);
+          rank += above(x.x, j) + above(x.y, j + 1) + above(x.z, j + 2) + above(x.w, j + 3);
+        }
+      };
+      const uint32_t w0 = 64u * wave;
+      count(0, w0, [&](uint32_t x, uint32_t) { return x >= mine ? 1u : 0u; });
+      count(w0, w0 + 64, [&](uint32_t x, uint32_t j) { return x > (j < tid ? mine - 1 : mine) ? 1u : 0u; });
+      count(w0 + 64, n, [&](uint32_t x, uint32_t) { return x > mine ? 1u : 0u; });
       ranked_take = free && rank < need;
     } else if (need == 0) {  // nothing but the forced ones: no key reaches the range
       lo = 0xFFFFFFFFu;
@@ -83,11 +113,8 @@ __device__ __forceinline__ void take_largest(const Key &key, uint32_t n, uint32_
         mn = min(mn, x);
         mx = max(mx, x);
       }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        mn = min(mn, static_cast<uint32_t>(__shfl_xor(mn, o)));
-        mx = max(mx, static_cast<uint32_t>(__shfl_xor(mx, o)));
-      }
+      mn = ~wave_max(~mn);
+      mx = wave_max(mx);
       if (lane == 0) {
         sh.wave[0][wave][0] = mn;
         sh.wave[0][wave][1] = mx;
