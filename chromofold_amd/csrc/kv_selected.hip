@@ -194,9 +194,81 @@ struct Query {
   }
 };
 
-// A wavefront's running state of one row: maximum and sum of the heads 4 b + r, sums of p v of the heads 4 b + r (row r of the
-// accumulators) at dim 16 i + n.
-template <int D>
+// How the softmax's work lies in the lanes. The scores come from the MFMAs with the heads 4 b + r in lane group b, a tile of
+// 16 tokens per accumulator: with at most 4 heads only one group of lanes has any, 16 of them each. GT = lane groups that the
+// heads fill (1, 2 or 4): with fewer than 4 the tiles are dealt out over the idle groups by row exchanges, and a lane
+// (b, n) keeps GT scores of each of the heads 4 (b % GT) + r, at the tokens token(j), j < GT. At 4 heads that takes the
+// vector instructions of a group from 465 to 366 at D = 64 and from 635 to 537 at D = 128 (32 x 512 groups of hd 64, 1.1 GB:
+// 217 -> 189 us).
+template <int GT>
+struct Spread {
+  // exchange of rows: {a0 b0 a2 b2, a1 b1 a3 b3} and {a0 a1 b0 b1, a2 a3 b2 b3}
+  static __device__ __forceinline__ void swap16(float &a, float &b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+  }
+  static __device__ __forceinline__ void swap32(float &a, float &b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+  }
+  static __device__ __forceinline__ uint32_t head(int b, int r) { return 4 * (b % GT) + r; }
+  static __device__ __forceinline__ int token(int n, int b, int j) { return 4 * n + (GT == 4 ? j : GT == 2 ? 2 * (b / 2) + j : b); }
+  // sc[i][r]: tile i, head 4 b + r -> s[j][r]
+  static __device__ __forceinline__ void deal(const float4_t (&sc)[4], float (&s)[GT][4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x[4] = {sc[0][r], sc[1][r], sc[2][r], sc[3][r]};
+      if constexpr (GT < 4) {
+        swap32(x[0], x[2]);
+        swap32(x[1], x[3]);
+      }
+      if constexpr (GT == 1) swap16(x[0], x[1]);
+#pragma unroll
+      for (int j = 0; j < GT; ++j) s[j][r] = x[j];
+    }
+  }
+  // Reduces x[r] over all lanes that hold the head of (b, r); every such lane gets the result.
+  template <typename Op, typename Row>
+  static __device__ __forceinline__ void reduce(float (&x)[4], const Op &op, const Row &row16) {
+    if constexpr (GT == 4) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = row16(x[r]);
+    } else {
+      swap32(x[0], x[1]);
+      swap32(x[2], x[3]);
+      float a = op(x[0], x[1]), c = op(x[2], x[3]);  // halves: heads of r = 0 | 1, and of r = 2 | 3
+      if constexpr (GT == 2) {
+        a = row16(a);
+        c = row16(c);
+        x[0] = x[1] = a;
+        x[2] = x[3] = c;
+        swap32(x[0], x[1]);
+        swap32(x[2], x[3]);
+      } else {
+        swap16(a, c);
+        a = row16(op(a, c));  // rows: r = 0, 2, 1, 3
+        x[0] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), 0));
+        x[1] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), 32));
+        x[2] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), 16));
+        x[3] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), 48));
+      }
+    }
+  }
+  // (fmaxf and not cfd::vmax_f32: a row exchange must not follow within two wait states of the write of what it exchanges,
+  // which the compiler sees to for its own instructions only)
+  static __device__ __forceinline__ void reduce_max(float (&x)[4]) {
+    reduce(x, [](float a, float b) { return fmaxf(a, b); }, [](float a) { return cfd::row16_max(a); });
+  }
+  static __device__ __forceinline__ void reduce_sum(float (&x)[4]) {
+    reduce(x, [](float a, float b) { return a + b; }, [](float a) { return cfd::row16_sum(a); });
+  }
+};
+
+// A wavefront's running state of one row: maximum and sum of the heads Spread::head(b, r), sums of p v of the heads 4 b + r
+// (row r of the accumulators) at dim 16 i + n.
+template <int D, int GT>
 struct RowState {
   float m[4], l[4];
   int e;  // acc holds sums in units of 2^e
@@ -226,7 +298,7 @@ struct RowState {
     const int x = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;
     const float u = ldexpf(a.d.softmax_scale * kLog2e, x);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) unit[r] = __shfl(u, 4 * b + r);
+    for (int r = 0; r < 4; ++r) unit[r] = __shfl(u, static_cast<int>(Spread<GT>::head(b, r)));
 #pragma unroll
     for (int s = 0; s < D / 32; ++s)
 #pragma unroll
@@ -261,26 +333,28 @@ struct RowState {
     }
     bad |= w.codec != CF_KV_CODEC_INT8 || w.dim != D;
     // tokens of a page are visible from its first on
-    const uint32_t page = 64 * g + 16 * (n >> 2), first = 64 * g + 4 * n, end = min(page + min(w.tc, 16u), visible);
-    const uint32_t nvis = end > first ? min(end - first, 4u) : 0u;
-    const bool page_vis = w.tc > 0 && page < visible;
+    const uint32_t page = 16 * (n >> 2), here = visible - 64 * g;  // g is a visible group
+    const uint32_t end = min(page + min(w.tc, 16u), here);         // of the page, in tokens of the group
+    const bool page_vis = w.tc > 0 && page < here;
     const float ks = w.ks, vs = w.vs;
     if (next) w.load_k(next);
     // ---- online softmax
-    float mx[4], p[4][4], sum[4];
+    float p[GT][4], mx[4], sum[4];
+    Spread<GT>::deal(sc, p);
     bool moved = false;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float f = unit[r] * ks;
+      float f = unit[r];
+      f *= ks;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i][r] = static_cast<uint32_t>(i) < nvis ? sc[i][r] * f : -INFINITY;
-      mx[r] = fmaxf(fmaxf(p[0][r], p[1][r]), fmaxf(p[2][r], p[3][r]));
-    }
+      for (int j = 0; j < GT; ++j) p[j][r] = static_cast<uint32_t>(Spread<GT>::token(n, b, j)) < end ? p[j][r] * f : -INFINITY;
+      mx[r] = p[0][r];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      mx[r] = cfd::row16_max(mx[r]);
-      moved |= mx[r] > m[r];
+      for (int j = 1; j < GT; ++j) mx[r] = fmaxf(mx[r], p[j][r]);
     }
+    Spread<GT>::reduce_max(mx);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) moved |= mx[r] > m[r];
     // units of the P.V sums: the exponent of the group's largest V scale among its visible pages, less 15, so that
     // weights p vs lie in [0, 2^15) and those down to 2^-29 of that are normal f16 numbers. Sums move to a larger unit
     // at once and to a smaller one when 2^8 below (a factor of a power of two; clamped so that it cannot overflow).
@@ -308,25 +382,42 @@ struct RowState {
     for (int r = 0; r < 4; ++r) {
       const float m0 = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i][r] = __builtin_amdgcn_exp2f(p[i][r] - m0);  // exp2(-inf) = 0
-      sum[r] = (p[0][r] + p[1][r]) + (p[2][r] + p[3][r]);
+      for (int j = 0; j < GT; ++j) p[j][r] = __builtin_amdgcn_exp2f(p[j][r] - m0);  // exp2(-inf) = 0
+      sum[r] = p[0][r];
+#pragma unroll
+      for (int j = 1; j < GT; ++j) sum[r] += p[j][r];
       l[r] += sum[r];
     }
     if (stats) {
+      Spread<GT>::reduce_sum(sum);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float t = cfd::row16_sum(sum[r]);
-        if (n == r && static_cast<uint32_t>(4 * b + r) < gqa) put(4 * b + r, m[r], t);
-      }
+      for (int r = 0; r < 4; ++r)
+        if (n == r && b < GT && static_cast<uint32_t>(4 * b + r) < gqa) put(4 * b + r, m[r], sum[r]);
     }
-    if (static_cast<uint32_t>(4 * b) < gqa) {
+    if (Spread<GT>::head(b, 0) < gqa) {
+      const int at = Spread<GT>::token(n, b, 0);
+      if constexpr (GT == 1) {
+        _Float16 h[4], lo[4];
+        cfd::split2_mul_f16(p[0][0], p[0][1], vsn, h[0], lo[0], h[1], lo[1]);
+        cfd::split2_mul_f16(p[0][2], p[0][3], vsn, h[2], lo[2], h[3], lo[3]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        _Float16 h0, l0, h1, l1, h2, l2, h3, l3;
-        cfd::split2_mul_f16(p[0][r], p[1][r], vsn, h0, l0, h1, l1);
-        cfd::split2_mul_f16(p[2][r], p[3][r], vsn, h2, l2, h3, l3);
-        *reinterpret_cast<half4_t *>(&lds.p[0][4 * b + r][4 * n]) = half4_t{h0, h1, h2, h3};
-        *reinterpret_cast<half4_t *>(&lds.p[1][4 * b + r][4 * n]) = half4_t{l0, l1, l2, l3};
+        for (int r = 0; r < 4; ++r) {
+          lds.p[0][r][at] = h[r];
+          lds.p[1][r][at] = lo[r];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          _Float16 h[GT], lo[GT];
+#pragma unroll
+          for (int j = 0; j < GT; j += 2) cfd::split2_mul_f16(p[j][r], p[j + 1][r], vsn, h[j], lo[j], h[j + 1], lo[j + 1]);
+          typedef _Float16 halves_t __attribute__((ext_vector_type(GT)));
+          halves_t hv, lv;
+#pragma unroll
+          for (int j = 0; j < GT; ++j) hv[j] = h[j], lv[j] = lo[j];
+          *reinterpret_cast<halves_t *>(&lds.p[0][Spread<GT>::head(b, r)][at]) = hv;
+          *reinterpret_cast<halves_t *>(&lds.p[1][Spread<GT>::head(b, r)][at]) = lv;
+        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -358,11 +449,10 @@ struct RowState {
   // and makes the sum a NaN).
   __device__ __forceinline__ void close() {
     const bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
+    Spread<GT>::reduce_sum(l);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      l[r] = cfd::row16_sum(l[r]);
+    for (int r = 0; r < 4; ++r)
       if (broken || l[r] != l[r]) m[r] = __builtin_nanf("");
-    }
   }
 
   // The closed state to memory, its sums in absolute units.
@@ -398,7 +488,7 @@ __device__ __forceinline__ void write_stats(float2 *__restrict__ to, const float
 }
 
 // kRow and kSplit: a workgroup takes slots of one row, its wavefronts a block of them each.
-template <int D, int W, bool ROW>
+template <int D, int W, bool ROW, int GT>
 __global__ __launch_bounds__(64 * W, 2) void row_kernel(SelArgs a) {
   __shared__ union {
     WaveLds wave[W];
@@ -425,7 +515,7 @@ __global__ __launch_bounds__(64 * W, 2) void row_kernel(SelArgs a) {
   const uint32_t visible = visible_tokens(a.d.seq_tokens[seq], a.d.query_pos[seq], a.d.max_groups);
   const uint32_t ngroups = (visible + 63) / 64, nslots = row_slots(a, ngroups);
   const uint32_t s0 = ROW ? 0 : min(split * a.per, nslots), s1 = ROW ? nslots : min(nslots, s0 + a.per);
-  RowState<D> st;
+  RowState<D, GT> st;
   st.reset();
   bool split_done = false, bad = false;
   // Slots are looked up 64 at a time (fewer where that many statistics would not fit), one a lane, so that no load of the
@@ -534,7 +624,7 @@ struct Stretch {
 
 // kSpan. A wavefront's stretch touches consecutive rows; it leaves one state for each of them, number wavefront + row in
 // the laid-out order (head * seq_count + sequence), which no other wavefront has, and a row's states lie side by side.
-template <int D>
+template <int D, int GT>
 __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
   constexpr int T = 64 * kWaves;
   __shared__ WaveLds s_wave[kWaves];
@@ -608,7 +698,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
   };
   auto lane_of = [](uint32_t x, int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(x, i)); };
 
-  RowState<D> st;
+  RowState<D, GT> st;
   st.reset();
   Blob<D> w;
   Look k{};
@@ -1074,23 +1164,26 @@ Plan make_plan(const cf_kv_batched_desc *d, const cf_kv_selection *s) {
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+template <int D, int GT>
+void launch_cut(const SelArgs &a, Mode mode, hipStream_t s) {
+  const uint32_t heads = a.d.kv_head_count, seqs = a.d.seq_count;
+  if (mode == kRow) row_kernel<D, kWavesRow, true, GT><<<dim3(1, heads, seqs), 64 * kWavesRow, 0, s>>>(a);
+  else if (mode == kSpan) span_kernel<D, GT><<<(a.nwaves + kWaves - 1) / kWaves, 64 * kWaves, 0, s>>>(a);
+  else row_kernel<D, kWaves, false, GT><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
+}
+
 template <int D>
 void launch(const SelArgs &a, Mode mode, hipStream_t s) {
-  const uint32_t heads = a.d.kv_head_count, seqs = a.d.seq_count;
-  if (mode == kRow) {
-    row_kernel<D, kWavesRow, true><<<dim3(1, heads, seqs), 64 * kWavesRow, 0, s>>>(a);
-    return;
-  }
+  const uint32_t heads = a.d.kv_head_count, seqs = a.d.seq_count, gqa = a.d.query_head_count / heads;
+  if (mode == kCoded) coded_kernel<D><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
+  else if (gqa <= 4) launch_cut<D, 1>(a, mode, s);
+  else if (gqa <= 8) launch_cut<D, 2>(a, mode, s);
+  else launch_cut<D, 4>(a, mode, s);
+  if (mode == kRow) return;
   const uint32_t parts = a.s.weights_out ? (a.d.max_groups + kJoinGroups - 1) / kJoinGroups : 0;
-  const dim3 join(heads, seqs, a.d.query_head_count / heads + parts);
-  if (mode == kSpan) {
-    span_kernel<D><<<(a.nwaves + kWaves - 1) / kWaves, 64 * kWaves, 0, s>>>(a);
-    join_kernel<D, true><<<join, kJoinThreads, 0, s>>>(a);
-  } else {
-    if (mode == kCoded) coded_kernel<D><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
-    else row_kernel<D, kWaves, false><<<dim3(a.splits, heads, seqs), 64 * kWaves, 0, s>>>(a);
-    join_kernel<D, false><<<join, kJoinThreads, 0, s>>>(a);
-  }
+  const dim3 join(heads, seqs, gqa + parts);
+  if (mode == kSpan) join_kernel<D, true><<<join, kJoinThreads, 0, s>>>(a);
+  else join_kernel<D, false><<<join, kJoinThreads, 0, s>>>(a);
 }
 
 }  // namespace
