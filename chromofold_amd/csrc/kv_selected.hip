@@ -1123,12 +1123,12 @@ Plan make_plan(const cf_kv_batched_desc *d, const cf_kv_selection *s) {
   const bool fits = static_cast<uint64_t>(p.slots) * gqa <= kRowStats;  // a row's statistics in LDS
   uint64_t states = 0;
   // us of a call with weights, 8 KV heads, head_dim 128, 4 query heads per KV head unless said, as kSpan / kRow / kSplit:
-  //   32 x 64 of up to 512 groups (list)     61.1 /  46.2 /  53.1      32 x 512 groups            341.3 / 320.7 / 350.9
-  //   1 x 32 groups (list)                   13.0 /  19.1 /  11.9      32 x 8..512 groups         182.0 / 234.4 / 210.9
-  //   16 x 64 groups, 8 query heads          41.2 /  36.0 /  36.8      1 x 512 groups              29.1 / 194.5 /  21.4
-  //   64 x 32 groups                         65.2 /  53.0 /  56.4      1 x 2048 groups             60.3 / 749.8 /  52.9
-  //   64 x 16..125 groups of hd 64           80.2 /  75.1 /  96.1      4 x 2048 groups            164.4 / 760.2 / 171.7
-  //   128 x 32 of 128 groups (list)         111.8 / 105.7 / 106.7      256 x 8..32 groups         158.1 / 147.1 / 146.4
+  //   32 x 64 of up to 512 groups (list)     60.7 /  45.5 /  52.7      32 x 512 groups            339.9 / 319.6 / 349.2
+  //   1 x 32 groups (list)                   12.6 /  17.7 /  11.6      32 x 8..512 groups         180.9 / 227.4 / 207.9
+  //   16 x 64 groups, 8 query heads          40.9 /  35.7 /  38.8      1 x 512 groups              28.9 / 180.9 /  20.9
+  //   64 x 32 groups                         64.8 /  51.7 /  55.7      1 x 2048 groups             59.2 / 702.1 /  52.1
+  //   64 x 16..125 groups of hd 64           77.6 /  70.3 /  91.1      4 x 2048 groups            162.4 / 718.3 / 170.0
+  //   128 x 32 of 128 groups (list)         110.8 / 103.0 / 106.2      256 x 8..32 groups         157.1 / 142.5 / 145.2
   // A row to a workgroup where a list makes the rows alike and they fill the chip once, or where they are many and even out
   // by themselves; stretches from 16 slots a resident wavefront on, where its state is small beside them; else splits.
   if (d->codec == CF_KV_CODEC_RANS_HYBRID) p.mode = kCoded;

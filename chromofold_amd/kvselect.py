@@ -84,6 +84,14 @@ def _call(name: str, device: torch.device, s: int, *args) -> None:
         A.check(fn(*args, s), name)
 
 
+def _on_device(device: torch.device, fn, *args):
+    """A host-side call (validation, workspace sizes) with the tensors' device as the current one: sizes go by its CUs."""
+    if device.type != "cuda" or device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
 def _with_workspace(desc, need: int, device: torch.device, stream) -> None:
     """Gives the descriptor a workspace for calls on `stream`, allocated for that stream."""
     if need:
@@ -181,7 +189,7 @@ def select_desc(kvb: kv.BatchedKv, bounds: KeyBounds, queries: torch.Tensor, que
                           kvb.seq_tokens.data_ptr(), query_pos.data_ptr(), queries.data_ptr(), units.data_ptr())
     d.held = (bounds, kvb.seq_tokens, query_pos, queries, units)
     A.check(A.lib().cf_kv_validate_select_desc(C.byref(d)), "cf_kv_validate_select_desc")
-    _with_workspace(d, int(A.lib().cf_kv_select_workspace_bytes(C.byref(d))), dev, stream)
+    _with_workspace(d, int(_on_device(dev, A.lib().cf_kv_select_workspace_bytes, C.byref(d))), dev, stream)
     return d
 
 
@@ -211,6 +219,8 @@ def attention_desc(kvb: kv.BatchedKv, queries: torch.Tensor, output: torch.Tenso
     _need(query_pos, "query_pos", torch.int32, (S,), dev)
     if units is not None:
         _need(units, "units", torch.int32, (S, H, units.shape[-1]), dev)
+        if units.numel() == 0:  # its address would be NULL, which stands for all groups
+            raise ValueError("units lists nothing: at least one entry a row is needed")
     if weights is not None:
         _need(weights, "weights", torch.float32, shape, dev)
     if weights_out is not None:
@@ -223,7 +233,8 @@ def attention_desc(kvb: kv.BatchedKv, queries: torch.Tensor, output: torch.Tenso
                                   0 if units is None else units.shape[2], _ptr(units), _ptr(weights), _ptr(weights_out), decay)
     d.held = (kvb, queries, output, query_pos, units, weights, weights_out, d.selection)
     A.check(A.lib().cf_kv_validate_selection(C.byref(d), C.byref(d.selection)), "cf_kv_validate_selection")
-    _with_workspace(d, int(A.lib().cf_kv_selected_workspace_bytes(C.byref(d), C.byref(d.selection))), dev, stream)
+    need = _on_device(dev, A.lib().cf_kv_selected_workspace_bytes, C.byref(d), C.byref(d.selection))
+    _with_workspace(d, int(need), dev, stream)
     return d
 
 

@@ -722,6 +722,46 @@ def test_a_step_in_a_graph(dev):
         assert torch.equal(w, w2)
 
 
+@pytest.mark.parametrize("S, H, longest", [(300, 2, 4096), (260, 2, 500)])
+def test_attention_of_ragged_batches_in_a_graph(dev, S, H, longest):
+    """The cuts by device-side lengths in a graph: replays follow the lengths, positions and lists of the moment, with eager
+    calls (their own workspaces) between them."""
+    import torch
+    from chromofold_amd import kvselect as ks
+    rng = np.random.default_rng(S)
+    lens = [int(x) for x in rng.integers(1, 200, S)]
+    lens[7] = longest
+    c = Case(dev, lens, H, 4, 64, 63)
+    q, pos, w = up(dev, c.q), up(dev, np.array(c.pos, np.uint32)), torch.rand(S, H, c.M, device=dev)
+    out, w_out, out2, w_out2 = torch.empty_like(q), torch.empty_like(w), torch.empty_like(q), torch.empty_like(w)
+    units = up(dev, c.lists(c.M, 1, 0.7))
+
+    def call(o, wo, u):
+        ks.attention(c.kvb, q, o, pos, c.scale, u, 1, w, wo, 0.5)
+
+    for u in (None, units):
+        call(out2, w_out2, u)
+        torch.cuda.synchronize()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream(dev)
+        with torch.cuda.stream(side):
+            graph.capture_begin()
+            call(out, w_out, u)
+            graph.capture_end()
+        for k in range(4):
+            cut = rng.integers(0, np.array(lens) + 1).astype(np.uint32)
+            cut[7] = longest - 100 * k
+            c.kvb.seq_tokens.copy_(up(dev, cut))
+            pos.copy_(up(dev, rng.integers(0, np.array(lens) + 50).astype(np.uint32)))
+            units.copy_(up(dev, c.lists(c.M, 1, 0.3 + 0.2 * k)))
+            out.fill_(float("nan"))
+            torch.cuda.synchronize()
+            graph.replay()
+            (torch.randn(1 << 20, device=dev) ** 2).sum().item()
+            call(out2, w_out2, u)
+            torch.cuda.synchronize()
+            assert torch.equal(out, out2) and torch.equal(w_out, w_out2) and torch.isfinite(out).all()
+
+
 def test_two_streams_with_one_descriptor(dev):
     import torch
     from chromofold_amd import kvselect as ks

@@ -165,6 +165,7 @@ def test_binding_checks_tensors():
         lambda: ks.attention_desc(kvb, q, q[:1], z(S), 1.0),
         lambda: ks.attention_desc(kvb, q, q, z(S), 1.0, weights_out=w[:, :, :4]),
         lambda: ks.attention_desc(kvb, q, q, z(S), 1.0, units=z(S, 1, 3)),
+        lambda: ks.attention_desc(kvb, q, q, z(S), 1.0, units=z(S, H, 0)),
         lambda: ks.evict_desc(kvb, w[:1], 2),
         lambda: ks.evict_desc(kvb, w, 2, ks.Evicted(z(S, H, M), z(S), w, b), bounds=None),
         lambda: ks.evict_desc(kvb, w, 2, ks.Evicted(z(S, H, M), z(S + 1))),
