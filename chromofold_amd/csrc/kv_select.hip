@@ -13,7 +13,7 @@ namespace {
 typedef int int4_t __attribute__((ext_vector_type(4)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kMaxGroups = 1u << 26;  // tables are shorter: 64 * max_groups fits 32 bits
+constexpr uint32_t kMaxGroups = 1u << 25;  // tables are shorter: 64 * max_groups fits 32 bits
 constexpr int kRows = 16;                  // query heads of one KV head an MFMA tile takes
 
 // Tokens of a sequence its query sees, and tokens its table can hold.

@@ -1213,10 +1213,10 @@ extern "C" cf_status cf_kv_validate_selection(const cf_kv_batched_desc *d, const
     if (w != CF_OK) return w;
   }
   if (d->max_groups == 0) return CF_ERR_INVALID_ARGUMENT;
-  if (d->max_groups >= 1u << 26) return CF_ERR_UNSUPPORTED;
+  if (d->max_groups >= 1u << 25) return CF_ERR_UNSUPPORTED;  // 64 * max_groups in 32 bits, join grids in z
   if (s->units) {
     if (s->max_units == 0 || (s->unit_groups != 1 && s->unit_groups != 2)) return CF_ERR_INVALID_ARGUMENT;
-    if (s->max_units >= 1u << 26) return CF_ERR_UNSUPPORTED;
+    if (s->max_units >= 1u << 25) return CF_ERR_UNSUPPORTED;
   }
   if (!std::isfinite(s->decay) || (s->weights_in && !s->weights_out)) return CF_ERR_INVALID_ARGUMENT;
   return CF_OK;

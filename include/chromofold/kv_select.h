@@ -13,6 +13,9 @@
  * evicted as one: unit_groups = 1 group, or unit_groups = 2, the groups 2u and 2u + 1, which share a rANS chain in a
  * RANS_HYBRID pool sealed with chain pairs (seal with continues = NULL to use single groups there).
  *
+ * Limits (beyond them CF_ERR_UNSUPPORTED): max_groups and a selection's max_units below 2^25, seq_count and kv_head_count up
+ * to 65535. Tokens past 64 * max_groups do not count.
+ *
  * Every array is device memory on the current device; calls are asynchronous on `stream`, allocate nothing and never
  * synchronise, and may be captured into a graph. Calls that may overlap need a workspace each. Results repeat bit for bit.
  */

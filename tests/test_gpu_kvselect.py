@@ -675,6 +675,57 @@ def test_steps_select_attend_evict(dev):
     assert np.abs(down(out) - full).max() <= 1e-3 * np.abs(full).max()
 
 
+@pytest.mark.parametrize("chained", [True, False])
+def test_coded_cache_after_an_eviction(dev, chained):
+    """A rANS cache cut back by its attention weights, as chain pairs or as groups of their own, and what both attention
+    calls and a selection make of the tables that remain; ragged sequences, one below the budget, one with a cut last page."""
+    import torch
+    from chromofold_amd import kvselect as ks
+    unit = 2 if chained else 1
+    lens = [64 * 41, 64 * 30 + 21, 300, 64 * 44 + 1]
+    c = coded(dev, lens, 2, 4, 128, 95, chained)
+    S, H, M = len(lens), 2, c.M
+    q, w, out = up(dev, c.q), torch.zeros(S, H, M, device=dev), torch.empty(c.q.shape, device=dev)
+    pos = up(dev, np.array(c.pos, np.uint32))
+    ks.attention(c.kvb, q, out, pos, c.scale, weights=w, weights_out=w)
+    weights = down(w)
+    dropped = torch.empty(S, H, M, dtype=torch.int32, device=dev)
+    budget = 20 // unit
+    ks.evict(c.kvb, w, budget, ks.Evicted(c.kvb.group_offsets, c.kvb.seq_tokens, w, None, dropped), unit_groups=unit,
+             keep_first=1, keep_last=2)
+    tokens, kept = [], {}
+    for s, t in enumerate(lens):
+        n = -(-t // 64)
+        m = -(-n // unit)
+        k = min(m, budget)
+        tokens.append(t - 64 * unit * (m - k))
+        for h in range(H):
+            x = np.zeros(m * unit, np.float32)
+            x[:n] = weights[s, h, :n]
+            units = R.pick_ref(x.reshape(m, unit).sum(1, dtype=np.float32), m, k, 1, 2)
+            at = (units[:, None] * unit + np.arange(unit)).ravel()
+            kept[s, h] = at[at < n]
+    assert down(c.kvb.seq_tokens).tolist() == tokens
+    assert (u32(dropped)[0] != R.NO_UNIT).sum(1).tolist() == [41 - len(kept[0, 0]), 41 - len(kept[0, 1])]
+    pick = lambda x, s, h: np.concatenate([x[s][h][64 * g: 64 * g + 64] for g in kept[s, h]])  # noqa: E731
+    k = [[pick(c.k, s, h) for h in range(H)] for s in range(S)]
+    v = [[pick(c.v, s, h) for h in range(H)] for s in range(S)]
+    at = [t - 1 for t in tokens]
+    pos.copy_(up(dev, np.array(at, np.uint32)))
+    o, _, mag, big, low = R.attend_ref(c.q, k, v, tokens, at, 4, c.scale, None, 1, M)
+    bound = R.tolerance(big, 128)[..., None] * mag + 2.0 ** -23 * np.abs(o) + low
+    ks.attention(c.kvb, q, out, pos, c.scale)
+    assert (np.abs(down(out) - o) <= bound).all()
+    c.kvb.attention(q, out, pos, c.scale)
+    from kv_helpers import head_err
+    assert head_err(down(out), o) <= 1e-3
+    lists = np.full((S, H, 3), R.NO_UNIT, np.uint32)
+    lists[:, :, :2] = [0, 2]
+    o, _, mag, big, low = R.attend_ref(c.q, k, v, tokens, at, 4, c.scale, lists, unit, M)
+    ks.attention(c.kvb, q, out, pos, c.scale, up(dev, lists), unit)
+    assert (np.abs(down(out) - o) <= R.tolerance(big, 128)[..., None] * mag + 2.0 ** -23 * np.abs(o) + low).all()
+
+
 def test_a_step_in_a_graph(dev):
     """Selection, attention with weights in place and eviction captured into a graph and replayed with eager work between
     the replays: every replay gives what the eager calls give on the same inputs."""

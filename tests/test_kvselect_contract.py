@@ -46,7 +46,7 @@ def select_desc(**change):
     ({"keep_first": 0xFFFFFFFF, "keep_last": 2}, INV), ({"keep_first": 0, "keep_last": 0}, OK),
     ({"keep_first": 4, "keep_last": 4}, OK), ({"head_dim": 64}, OK), ({"head_dim": 96}, UNS), ({"query_head_count": 64}, OK),
     ({"query_head_count": 68}, UNS), ({"seq_count": 65536}, UNS), ({"kv_head_count": 65536, "query_head_count": 65536}, UNS),
-    ({"max_groups": 1 << 26}, UNS), ({"max_units": 1000}, OK),
+    ({"max_groups": 1 << 25}, UNS), ({"max_groups": (1 << 25) - 1}, OK), ({"max_units": 1000}, OK),
 ])
 def test_select_refusals(change, want):
     L, d = A.lib(), select_desc(**change)
@@ -80,12 +80,12 @@ def attention_args(desc=None, sel=None):
     ({}, {}, OK), ({}, {"struct_size": 4}, INV), ({}, {"abi_version": 0}, INV), ({}, {"units": None, "unit_groups": 7}, OK),
     ({}, {"max_units": 0}, INV), ({}, {"unit_groups": 0}, INV), ({}, {"unit_groups": 2}, OK), ({}, {"unit_groups": 4}, INV),
     ({}, {"weights_in": None}, OK), ({}, {"weights_in": None, "weights_out": None}, OK), ({}, {"weights_out": None}, INV),
-    ({}, {"decay": float("nan")}, INV), ({}, {"decay": float("inf")}, INV), ({}, {"max_units": 1 << 26}, UNS),
+    ({}, {"decay": float("nan")}, INV), ({}, {"decay": float("inf")}, INV), ({}, {"max_units": 1 << 25}, UNS),
     ({"struct_size": 0}, {}, INV), ({"pool": None}, {}, INV), ({"pool": P + 8}, {}, INV), ({"output": None}, {}, INV),
     ({"query_head_count": 64}, {}, OK), ({"query_head_count": 68}, {}, UNS), ({"query_head_count": 17}, {}, INV),
     ({"query_head_count": 64, "head_dim": 80}, {}, UNS), ({"head_dim": 64}, {}, OK), ({"head_dim": 32}, {}, UNS),
     ({"query_head_count": 64, "queries": None}, {}, INV), ({"query_head_count": 64, "seq_count": 65536}, {}, UNS),
-    ({"max_groups": 0}, {}, INV), ({"max_groups": 1 << 26}, {}, UNS), ({"softmax_scale": float("inf")}, {}, INV),
+    ({"max_groups": 0}, {}, INV), ({"max_groups": 1 << 25}, {}, UNS), ({"softmax_scale": float("inf")}, {}, INV),
     ({"codec": 3}, {}, UNS), ({"codec": kv.CODEC_RANS_HYBRID, "query_head_count": 20}, {}, UNS),
     ({"codec": kv.CODEC_RANS_HYBRID, "tables": None}, {}, INV),
 ])
@@ -128,7 +128,7 @@ NO_RECORDS = {"codes": None, "scales": None, "codes_out": None, "scales_out": No
     ({"keep_last": 0}, INV), ({"keep_first": 8}, INV), ({"keep_first": 7}, OK), ({"keep_last": 9}, INV),
     ({"codes": None}, INV), ({"scales_out": None}, INV), ({"codes": P + 4}, INV), ({"codes_out": P + 4}, INV),
     ({"head_dim": 256}, UNS), ({"head_dim": 64}, OK), ({"seq_count": 65536}, UNS), ({"kv_head_count": 65536}, UNS),
-    ({"max_groups": 1 << 26}, UNS),
+    ({"max_groups": 1 << 25}, UNS), ({"max_groups": (1 << 25) - 1}, OK),
 ])
 def test_evict_refusals(change, want):
     L, d = A.lib(), evict_desc(**change)
