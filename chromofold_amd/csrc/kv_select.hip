@@ -112,8 +112,8 @@ __global__ __launch_bounds__(64 * kBoundWaves) void key_bounds_kernel(
 
 // ---- selection --------------------------------------------------------------------------------------------------
 // Scores of 16 groups at a time on v_mfma_i32_16x16x64_i8: rows = the KV head's query heads, columns = groups, k = the 2 D
-// products of one group, [max(a, 0), max(-a, 0)] . [upper codes, negated lower codes]. A group's record is read by four
-// lanes in 16-byte pieces, every line of it whole within one step of the wavefront.
+// products of one group, [max(a, 0), max(-a, 0)] . [upper codes, negated lower codes]. Whole numbers: a score does not depend
+// on the order of its sum.
 template <int D>
 __device__ __forceinline__ void stage_query(const cf_kv_select_desc &d, uint32_t seq, uint32_t head, int8_t (*s_a)[2 * D],
                                             float *s_step, int nthreads) {
@@ -128,8 +128,7 @@ __device__ __forceinline__ void stage_query(const cf_kv_select_desc &d, uint32_t
       q[j] = static_cast<uint32_t>(h) < gqa ? row[lane + 64 * j] : 0.0f;
       top = fmaxf(top, fabsf(q[j]));
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    top = cfd::rows4_max(cfd::row16_max(top));
     const float step = top / 127.0f;
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
@@ -144,7 +143,7 @@ __device__ __forceinline__ void stage_query(const cf_kv_select_desc &d, uint32_t
 
 // Records of the 16 groups of a tile. Read as they lie, 1 KiB a wavefront load, and brought to the layout of a B operand
 // (lane (kb, n): quarters of group n) through LDS: loads in that layout touch 64 lines each, at which one CU's cache gives
-// 34 GB/s (2048 groups of a row 22 us, against 12 so).
+// 34 GB/s (a call of 8 rows of 2048 groups, one workgroup each, 22.7 us so, 16.5 through LDS).
 template <int D>
 struct Tile {
   static constexpr int kLoads = 2 * D / 64;
@@ -337,9 +336,9 @@ uint32_t row_units(const cf_kv_select_desc *d) { return (d->max_groups + d->unit
 
 // Threads of the one workgroup that takes a row, 0 for two launches (scores of a row over many workgroups, then the pick).
 // us at 32 query / 8 KV heads, head_dim 128, as 256 threads / 1024 threads / two launches:
-//   rows x groups      8 x 128    8.2 /  8.7 / 11.2      8 x 1024  16.4 / 12.2 / 11.8      32 x 2048  25.7 / 16.7 / 15.9
-//                    256 x 512   12.0 / 11.2 / 15.9    128 x 2048  26.6 / 19.2 / 22.2     256 x 2048  30.7 / 27.8 / 32.5
-//                    512 x 128   10.2 / 16.5 / 18.3   1024 x 128   15.8 / 31.0 / 25.6    1024 x 512   26.6 / 47.7 / 40.4
+//   rows x groups      8 x 128    6.6 /  7.5 / 10.3      8 x 1024  14.8 / 11.1 / 10.8      32 x 2048  23.8 / 15.5 / 14.6
+//                    256 x 512   12.4 / 13.2 / 16.3    128 x 2048  24.7 / 18.1 / 20.6     256 x 2048  29.3 / 26.8 / 31.0
+//                    512 x 128    9.3 / 14.7 / 18.1   1024 x 128   12.9 / 26.7 / 26.6    1024 x 512   25.4 / 44.2 / 42.2
 // Workgroups of 256 threads leave several a CU: for more rows than CUs, and for rows too short to keep more wavefronts busy.
 // One CU reads a row at some 70 GB/s, which loses to two launches when the row is long and other CUs would be idle.
 int row_threads(const cf_kv_select_desc *d) {
@@ -431,7 +430,8 @@ __global__ __launch_bounds__(T) void evict_kernel(cf_kv_evict_desc d, bool token
             for (uint32_t e = 0; e < kPer; ++e) {
               const uint32_t p = e * T + tid;
               if (p < m)
-                v[e] = *reinterpret_cast<const int4_t *>(d.codes + (row + s_from[(a + p / kL) % (2 * T)]) * (2 * D) + 16 * (p % kL));
+                v[e] = *reinterpret_cast<const int4_t *>(d.codes + (row + s_from[(a + p / kL) % (2 * T)]) * (2 * D) +
+                                                         16 * (p % kL));
             }
           }
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every read of this wavefront has returned

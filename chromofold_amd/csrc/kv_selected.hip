@@ -125,8 +125,9 @@ __device__ __forceinline__ float group_weight(const Stat &stat, uint32_t gqa, co
 
 // The row's weights of groups [lo, hi): decayed, then the listed ones' shares added. All threads of the workgroup call this.
 template <typename Stat>
-__device__ __forceinline__ void write_weights(const SelArgs &a, size_t row, const uint32_t *list, uint32_t ngroups, uint32_t nslots,
-                                              uint32_t lo, uint32_t hi, uint32_t gqa, const float *m, const float *inv_l, const Stat &stat) {
+__device__ __forceinline__ void write_weights(const SelArgs &a, size_t row, const uint32_t *list, uint32_t ngroups,
+                                              uint32_t nslots, uint32_t lo, uint32_t hi, uint32_t gqa, const float *m,
+                                              const float *inv_l, const Stat &stat) {
   const float *in = a.s.weights_in ? a.s.weights_in + row * a.d.max_groups : nullptr;
   float *out = a.s.weights_out + row * a.d.max_groups;
   if (!list) {
@@ -475,7 +476,8 @@ __device__ __forceinline__ const uint8_t *blob_at(const SelArgs &a, uint32_t off
 }
 
 // Statistics of `count` slots looked up together from the wavefront's LDS to memory; `dest`: the place of this lane's slot.
-__device__ __forceinline__ void write_stats(float2 *__restrict__ to, const float2 *stat, uint32_t dest, uint32_t count, uint32_t gqa) {
+__device__ __forceinline__ void write_stats(float2 *__restrict__ to, const float2 *stat, uint32_t dest, uint32_t count,
+                                            uint32_t gqa) {
   const uint32_t lane = threadIdx.x & 63;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -756,8 +758,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
 // ---- RANS_HYBRID pools: the batched decode's group body (kv_group_body.hpp; at most 4 query heads per KV head), groups of a
 // unit decoded back to back by one wavefront, since a chain may run across them. Bound by the entropy decode, as there: the
 // tables are staged by every workgroup and the memory pipeline restarts at every row. 32 pairs of 512 groups for each of
-// 32 x 8 rows (252 MB) 68 us, all their 512 groups (2.02 GB) 477, 462 without weights (kv_batched.hip 374-396). Two wavefronts a SIMD: at three the
-// code for raw groups beside the lookups spills (75 and 478 us with 13 registers spilled, 111 and 622 with 58).
+// 32 x 8 rows (252 MB) 68 us, all their 512 groups (2.02 GB) 477, 462 without weights (kv_batched.hip 374-396). Two
+// wavefronts a SIMD: at three the code for raw groups beside the lookups spills (81 and 484 us with 13 registers spilled,
+// 111 and 622 with 58).
 
 // A unit's groups in this launch: the list's units, or pairs (a chain never spans more).
 __host__ __device__ inline uint32_t coded_item(const cf_kv_selection &s) { return s.units ? s.unit_groups : 2u; }
@@ -1050,9 +1053,10 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a, uint32_t 
   // the sums of this thread's first states, in flight while the maxima are found
   float o8[kB];
 #pragma unroll
-  for (uint32_t u = 0; u < kB; ++u)
-    o8[u] = out && states ? sums[static_cast<size_t>(min(part + u * parts, states - 1)) * gqa * D + e0 + (every ? min(tid, en - 1) : tid % D)]
-                          : 0.0f;
+  for (uint32_t u = 0; u < kB; ++u) {
+    const uint32_t e = e0 + (every ? min(tid, en - 1) : tid % D);
+    o8[u] = out && states ? sums[static_cast<size_t>(min(part + u * parts, states - 1)) * gqa * D + e] : 0.0f;
+  }
   // a wavefront per query head: its maximum and the inverse of its sum
   for (uint32_t h = every ? tid >> 6 : blockIdx.z; h < (every ? gqa : blockIdx.z + 1); h += kJoinThreads / 64) {
     float m = -INFINITY, l = 0.0f;

@@ -141,8 +141,9 @@ def key_bounds(keys: torch.Tensor, first_page: torch.Tensor, page_counts: torch.
     _need(out.scales, "out.scales", torch.float32, rows, dev)
     _need(out.codes, "out.codes", torch.int8, (*rows, 2 * D), dev)
     if n:
-        _call("cf_kv_key_bounds_async", dev, _raw_stream(dev, stream), keys.data_ptr(), n, first_page.data_ptr(), page_counts.data_ptr(),
-              _ptr(token_counts), D, _ptr(slots), out.codes.data_ptr(), out.scales.data_ptr(), out.scales.numel())
+        _call("cf_kv_key_bounds_async", dev, _raw_stream(dev, stream), keys.data_ptr(), n, first_page.data_ptr(),
+              page_counts.data_ptr(), _ptr(token_counts), D, _ptr(slots), out.codes.data_ptr(), out.scales.data_ptr(),
+              out.scales.numel())
     return out
 
 
@@ -198,7 +199,8 @@ def select(kvb: kv.BatchedKv, bounds: KeyBounds, queries: torch.Tensor, query_po
            desc: cf_kv_select_desc | None = None) -> torch.Tensor:
     """Fills units int32 [seq_count, kv_heads, max_units] with the units of each row whose bound on the scores of `queries`
     [seq_count, query_heads, D] is largest, the first keep_first and the last keep_last always, ascending, then NO_UNIT."""
-    d = desc if desc is not None else select_desc(kvb, bounds, queries, query_pos, units, unit_groups, keep_first, keep_last, stream)
+    d = desc if desc is not None else select_desc(kvb, bounds, queries, query_pos, units, unit_groups, keep_first,
+                                                  keep_last, stream)
     dev = kvb.group_offsets.device
     s = _raw_stream(dev, stream)
     _call("cf_kv_select_groups_async", dev, s, C.byref(_for_stream(d, cf_kv_select_desc, dev, stream, s)))

@@ -96,10 +96,11 @@ cf_status cf_kv_select_groups_async(const cf_kv_select_desc *desc, void *stream)
 /* ---- attention over selected groups ------------------------------------------------------------------------------
  * cf_kv_paged_attention_batched_async over the listed units of each (sequence, KV head). units [seq_count, kv_head_count,
  * max_units] ascends strictly up to the first CF_KV_NO_UNIT, which only CF_KV_NO_UNIT follows, as
- * cf_kv_select_groups_async writes it; a row that does not becomes NaN (its output, and the
- * weights of the groups it lists). Of a row the first min(max_units, n) entries are read, n being its units with a visible
- * token: more cannot be listed. Units without a visible token are passed over; units = NULL takes every group (max_units and unit_groups are then ignored). Rows with nothing to
- * attend are 0.
+ * cf_kv_select_groups_async writes it; a row that does not becomes NaN (its output, and the weights of the groups it
+ * lists). Of a row the first min(max_units, n) entries are read, n being its units with a visible token: more cannot be
+ * listed. Units without a visible token are passed over; units = NULL takes every group (max_units and unit_groups are then
+ * ignored). Rows with nothing to attend are 0. As in the batched call, with splits = 0 a row's fp32 rounding may depend on
+ * the other rows' lengths.
  *
  * weights_out (may be NULL), per group, is fp32: weights_out = decay * weights_in + the softmax weight of the group's
  * tokens summed over the KV head's query heads (0 for a group not attended). All max_groups entries of a row are written.
