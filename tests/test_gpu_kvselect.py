@@ -537,11 +537,11 @@ def _evict(dev, x, tokens, unit, budget, first, last, D, place, records=True):
     kvb = kv.BatchedKv(kv.CODEC_INT8, S, H, D, M, torch.zeros(16, dtype=torch.uint8, device=dev), off, tok, None)
     b = ks.KeyBounds(up(dev, x["codes"]), up(dev, x["scales"])) if records else None
     dropped = torch.full((S, H, M), 5, dtype=torch.int32, device=dev)
-    if place:
-        to = ks.Evicted(off, tok, w, b, dropped)
-    else:
-        to = ks.Evicted(torch.full_like(off, 77), torch.full_like(tok, 77), torch.full_like(w, 77),
-                        ks.KeyBounds(torch.full_like(b.codes, 77), torch.full_like(b.scales, 77)) if records else None, dropped)
+    # place: which outputs are the inputs of their kind (True: all)
+    same = {"offsets", "tokens", "weights", "records"} if place is True else set() if place is False else {place}
+    other = lambda t, name: t if name in same else torch.full_like(t, 77)
+    to = ks.Evicted(other(off, "offsets"), other(tok, "tokens"), other(w, "weights"),
+                    ks.KeyBounds(other(b.codes, "records"), other(b.scales, "records")) if records else None, dropped)
     ks.evict(kvb, w, budget, to, bounds=b, unit_groups=unit, keep_first=first, keep_last=last)
     ref = _evict_ref(x, tokens, unit, budget, first, last, M)
     assert np.array_equal(down(to.seq_tokens).view(np.uint32), ref["tokens"])
@@ -550,13 +550,13 @@ def _evict(dev, x, tokens, unit, budget, first, last, D, place, records=True):
     for (s, h), at in ref["at"].items():
         n = at.size
         assert np.array_equal(go[s, h, :n], x["offsets"][s, h, at])
-        assert np.array_equal(go[s, h, n:], x["offsets"][s, h, n:] if place else np.full(M - n, 77))
+        assert np.array_equal(go[s, h, n:], x["offsets"][s, h, n:] if "offsets" in same else np.full(M - n, 77))
         assert np.array_equal(gw[s, h, :n], x["weights"][s, h, at], equal_nan=True) and (gw[s, h, n:] == 0).all()
         if records:
             gc, gs = down(to.bounds.codes)[s, h], down(to.bounds.scales)[s, h]
             assert np.array_equal(gc[:n], x["codes"][s, h, at]) and np.array_equal(gs[:n], x["scales"][s, h, at])
-            assert np.array_equal(gc[n:], x["codes"][s, h, n:] if place else np.full_like(gc[n:], 77))
-            assert np.array_equal(gs[n:], x["scales"][s, h, n:] if place else np.full_like(gs[n:], 77))
+            assert np.array_equal(gc[n:], x["codes"][s, h, n:] if "records" in same else np.full_like(gc[n:], 77))
+            assert np.array_equal(gs[n:], x["scales"][s, h, n:] if "records" in same else np.full_like(gs[n:], 77))
 
 
 def _tables(rng, S, H, M, D):
@@ -600,6 +600,19 @@ def test_evict_weights_out_of_the_ordinary(dev):
 def test_evict_long(dev):
     x = _tables(np.random.default_rng(10), 1, 2, 20000, 64)
     _evict(dev, x, [64 * 20000 - 5], 1, 12345, 10, 100, 64, True)
+    _evict(dev, x, [64 * 20000 - 5], 1, 12345, 10, 100, 64, False)
+    _evict(dev, x, [64 * 20000 - 5], 2, 5001, 10, 100, 64, False)
+
+
+@pytest.mark.parametrize("place", ["offsets", "tokens", "weights", "records"])
+@pytest.mark.parametrize("S, H, M, unit, budget", [(1, 1, 3000, 1, 1500), (3, 2, 2500, 2, 701), (5, 3, 90, 1, 41),
+                                                   (16, 8, 300, 1, 130), (20, 13, 70, 2, 20)])
+def test_evict_some_arrays_in_place(dev, place, S, H, M, unit, budget):
+    # few rows are moved by several workgroups each, unless one of them reads what another one writes
+    rng = np.random.default_rng(S + M)
+    x = _tables(rng, S, H, M, 128)
+    tokens = [64 * M - int(v) for v in rng.integers(0, 64 * (M // 3), S)]
+    _evict(dev, x, tokens, unit, budget, 1, 2, 128, place)
 
 
 # ---------------------------------------------------------------------------------------------------- together
