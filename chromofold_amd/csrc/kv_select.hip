@@ -150,10 +150,12 @@ struct Tile {
   static constexpr int kStride = 2 * D + 16;  // of a record in LDS: the 16 lanes of a read lie in different banks
   int4_t b[kLoads];
   float scale;  // of group n
-  __device__ __forceinline__ void load(const int8_t *__restrict__ codes, const float *__restrict__ scales, uint32_t tile,
-                                       uint32_t ngroups) {
+  // ngroups: of the row that may be read
+  __device__ __forceinline__ void load(const cf_kv_select_desc &d, size_t row, uint32_t tile, uint32_t ngroups) {
     constexpr int kL = 2 * D / 16;  // lanes of a record
     const int lane = threadIdx.x & 63;
+    const int8_t *__restrict__ codes = d.codes + row * d.max_groups * (2 * D);
+    const float *__restrict__ scales = d.scales + row * d.max_groups;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const size_t g = min(16 * tile + j * (64 / kL) + lane / kL, ngroups - 1);
@@ -212,22 +214,14 @@ struct QueryOperand {
 };
 
 // Scores of the tiles wave0, wave0 + nwaves, ... of a row; put(unit, key) receives them. Two tiles at a time, the next
-// ones' records loaded into their registers as soon as the products are formed (8 KiB a wavefront in flight at D = 128); the
-// first ones' before the queries are staged. All threads of the workgroup call this.
+// ones' records loaded into their registers as soon as the products are formed (8 KiB a wavefront in flight at D = 128). The
+// caller has loaded the first two, t, and staged the queries. All threads of the workgroup call this.
 template <int D, typename Put>
-__device__ __forceinline__ void score_row(const cf_kv_select_desc &d, uint32_t seq, uint32_t head, uint32_t ngroups, uint32_t wave0,
-                                          uint32_t nwaves, int nthreads, int8_t (*s_a)[2 * D], float *s_step,
+__device__ __forceinline__ void score_row(const cf_kv_select_desc &d, size_t row, uint32_t ngroups, uint32_t wave0,
+                                          uint32_t nwaves, Tile<D> (&t)[2], const int8_t (*s_a)[2 * D], const float *s_step,
                                           int8_t (*s_rec)[16 * Tile<D>::kStride], const Put &put) {
-  const size_t row = static_cast<size_t>(seq) * d.kv_head_count + head;
-  const int8_t *codes = d.codes + row * d.max_groups * (2 * D);
-  const float *scales = d.scales + row * d.max_groups;
   const uint32_t tiles = (ngroups + 15) / 16, unit = d.unit_groups, gqa = d.query_head_count / d.kv_head_count;
   const int lane = threadIdx.x & 63;
-  Tile<D> t[2];
-#pragma unroll
-  for (uint32_t j = 0; j < 2; ++j)
-    if (wave0 + j * nwaves < tiles) t[j].load(codes, scales, wave0 + j * nwaves, ngroups);
-  stage_query<D>(d, seq, head, s_a, s_step, nthreads);
   __syncthreads();
   QueryOperand<D> q;
   q.load(s_a, s_step);
@@ -238,7 +232,7 @@ __device__ __forceinline__ void score_row(const cf_kv_select_desc &d, uint32_t s
     for (uint32_t j = 0; j < 2; ++j) {
       c[j] = t[j].products(q.a, s_rec[threadIdx.x >> 6]);
       scale[j] = t[j].scale;
-      if (i + (j + 2) * nwaves < tiles) t[j].load(codes, scales, i + (j + 2) * nwaves, ngroups);
+      if (i + (j + 2) * nwaves < tiles) t[j].load(d, row, i + (j + 2) * nwaves, ngroups);
     }
 #pragma unroll
     for (uint32_t j = 0; j < 2; ++j) {
@@ -272,7 +266,7 @@ __device__ __forceinline__ uint32_t visible_units(const cf_kv_select_desc &d, ui
 }
 
 // A row's scores and its best units in one workgroup of T threads, the keys in LDS: grid (KV heads, sequences).
-constexpr uint32_t row_units_most(int T) { return T == 1024 ? 8192 : 2048; }
+constexpr uint32_t row_units_most(int T) { return T == 1024 ? 8192 : T == 512 ? 4096 : 2048; }
 
 template <int D, int T>
 __global__ __launch_bounds__(T) void select_row_kernel(cf_kv_select_desc d) {
@@ -282,21 +276,30 @@ __global__ __launch_bounds__(T) void select_row_kernel(cf_kv_select_desc d) {
   __shared__ __attribute__((aligned(16))) int8_t s_rec[T / 64][16 * Tile<D>::kStride];
   __shared__ cfsel::TopkShared<T> sh;
   const uint32_t head = blockIdx.x, seq = blockIdx.y;
-  const uint32_t ngroups = (visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups) + 63) / 64;
+  const uint32_t tokens = d.seq_tokens[seq], pos = d.query_pos[seq], wave = threadIdx.x >> 6;
+  const size_t row = static_cast<size_t>(seq) * d.kv_head_count + head;
+  // The first tiles and the queries do not wait for the row's length; what lies behind it is read for nothing (256 rows
+  // x 512 groups 11.8 -> 11.0 us).
+  Tile<D> t[2];
+  t[0].load(d, row, wave, d.max_groups);
+  stage_query<D>(d, seq, head, s_a, s_step, T);
+  const uint32_t ngroups = (visible_tokens(tokens, pos, d.max_groups) + 63) / 64;
   const uint32_t n = visible_units(d, ngroups);
   if (n > d.max_units) {
-    score_row<D>(d, seq, head, ngroups, threadIdx.x >> 6, T / 64, T, s_a, s_step, s_rec, [&](uint32_t u, uint32_t key) {
+    if (16 * (wave + T / 64) < ngroups) t[1].load(d, row, wave + T / 64, ngroups);
+    score_row<D>(d, row, ngroups, wave, T / 64, t, s_a, s_step, s_rec, [&](uint32_t u, uint32_t key) {
       if (u < n) s_key[u] = key;
     });
     __syncthreads();
   }
-  pick_units<T>(d, static_cast<size_t>(seq) * d.kv_head_count + head, n, s_key, sh);
+  pick_units<T>(d, row, n, s_key, sh);
 }
 
 template <int D>
 void launch_rows(const cf_kv_select_desc &d, int threads, hipStream_t s) {
   const dim3 grid(d.kv_head_count, d.seq_count);
   if (threads == 1024) select_row_kernel<D, 1024><<<grid, 1024, 0, s>>>(d);
+  else if (threads == 512) select_row_kernel<D, 512><<<grid, 512, 0, s>>>(d);
   else select_row_kernel<D, 256><<<grid, 256, 0, s>>>(d);
 }
 
@@ -313,11 +316,17 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(cf_kv_select_desc 
   const uint32_t ngroups = (visible_tokens(d.seq_tokens[seq], d.query_pos[seq], d.max_groups) + 63) / 64;
   constexpr uint32_t kPer = kScoreThreads / 64;
   if (16 * blockIdx.x * kPer >= ngroups) return;
-  uint32_t *out = keys + (static_cast<size_t>(seq) * d.kv_head_count + head) * row_units;
-  score_row<D>(d, seq, head, ngroups, blockIdx.x * kPer + (threadIdx.x >> 6), gridDim.x * kPer, kScoreThreads, s_a, s_step, s_rec,
-               [&](uint32_t u, uint32_t key) {
-                 if (u < row_units) out[u] = key;
-               });
+  const size_t row = static_cast<size_t>(seq) * d.kv_head_count + head;
+  uint32_t *out = keys + row * row_units;
+  const uint32_t wave0 = blockIdx.x * kPer + (threadIdx.x >> 6), nwaves = gridDim.x * kPer;
+  Tile<D> t[2];
+#pragma unroll
+  for (uint32_t j = 0; j < 2; ++j)
+    if (16 * (wave0 + j * nwaves) < ngroups) t[j].load(d, row, wave0 + j * nwaves, ngroups);
+  stage_query<D>(d, seq, head, s_a, s_step, kScoreThreads);
+  score_row<D>(d, row, ngroups, wave0, nwaves, t, s_a, s_step, s_rec, [&](uint32_t u, uint32_t key) {
+    if (u < row_units) out[u] = key;
+  });
 }
 
 // ... and the best units of each row from there: grid (KV heads, sequences).
@@ -335,19 +344,22 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(cf_kv_select_desc d,
 uint32_t row_units(const cf_kv_select_desc *d) { return (d->max_groups + d->unit_groups - 1) / d->unit_groups; }
 
 // Threads of the one workgroup that takes a row, 0 for two launches (scores of a row over many workgroups, then the pick).
-// us at 32 query / 8 KV heads, head_dim 128, as 256 threads / 1024 threads / two launches:
-//   rows x groups      8 x 128    6.6 /  7.5 / 10.3      8 x 1024  14.8 / 11.1 / 10.8      32 x 2048  23.8 / 15.5 / 14.6
-//                    256 x 512   12.4 / 13.2 / 16.3    128 x 2048  24.7 / 18.1 / 20.6     256 x 2048  29.3 / 26.8 / 31.0
-//                    512 x 128    9.3 / 14.7 / 18.1   1024 x 128   12.9 / 26.7 / 26.6    1024 x 512   25.4 / 44.2 / 42.2
-// Workgroups of 256 threads leave several a CU: for more rows than CUs, and for rows too short to keep more wavefronts busy.
-// One CU reads a row at some 70 GB/s, which loses to two launches when the row is long and other CUs would be idle.
+// us at 32 query / 8 KV heads, head_dim 128, as 256 / 512 / 1024 threads / two launches:
+//   rows x groups   8 x 64     5.9 /  5.6 /  6.1 /  9.6     8 x 512  10.2 /  8.3 /  9.1 / 10.5     8 x 1024 15.0 / 10.8 / 10.9 / 10.8
+//                   8 x 2048  24.2 / 16.4 / 15.1 / 11.9    32 x 2048 25.1 / 17.0 / 15.4 / 14.7    64 x 2048 27.6 / 18.0 / 15.7 / 17.7
+//                 256 x 64     6.0 /  5.7 /  6.1 /  9.8   256 x 512  11.9 / 11.0 / 12.1 / 16.3   256 x 2048 33.1 / 26.1 / 25.7 / 31.0
+//                 512 x 128    8.9 / 10.4 / 15.1 / 17.9   512 x 512  16.4 / 15.3 / 21.3 / 23.9   512 x 1024 27.1 / 25.4 / 29.1 / 34.8
+//                1024 x 128   12.2 / 17.0 / 27.4 / 27.0  1024 x 256  15.8 / 18.5 / 33.5 / 30.2  1024 x 512  25.8 / 26.7 / 38.1 / 42.2
+// Small workgroups leave several a CU, for more rows than CUs; a long row is read faster by many wavefronts, but one CU reads
+// it at some 70 GB/s at best, which loses to two launches when other CUs would be idle.
 int row_threads(const cf_kv_select_desc *d) {
   const uint32_t units = row_units(d);
-  const uint64_t rows = static_cast<uint64_t>(d->seq_count) * d->kv_head_count;
+  const bool many = static_cast<uint64_t>(d->seq_count) * d->kv_head_count > cfd::cu_count();
+  const bool few = static_cast<uint64_t>(d->seq_count) * d->kv_head_count < 64;
   const uint64_t row_bytes = static_cast<uint64_t>(d->max_groups) * 2 * d->head_dim;
-  if (units <= row_units_most(256) && (rows > cfd::cu_count() || row_bytes <= (32u << 10))) return 256;
-  if (units <= row_units_most(1024) && (rows >= 64 || row_bytes <= (256u << 10))) return 1024;
-  return 0;
+  if (units > row_units_most(1024) || (few && row_bytes > (256u << 10))) return 0;
+  if (many && d->max_groups <= 256) return 256;
+  return units <= row_units_most(512) && (many || d->max_groups <= 1024) ? 512 : 1024;
 }
 
 // ---- eviction ---------------------------------------------------------------------------------------------------
@@ -465,7 +477,7 @@ __global__ __launch_bounds__(T) void evict_kernel(cf_kv_evict_desc d, bool token
 }
 
 // Workgroups of a row: each picks all of it and moves its part of what stays, where no array is written that they read and
-// CUs would be idle (one of 1024 threads fits a CU). us with 1 / 2 / 4 / 8 / 16 of them: 32 rows, 1024 of 2048 groups
+// CUs would be idle (one of 1024 threads fits a CU). us, of 1024 threads, with 1 / 2 / 4 / 8 / 16 of them: 32 rows, 1024 of 2048 groups
 // 15.1 / 12.4 / 11.3 / 10.9 / 17.9; 8 rows, 64 of 128 groups 6.3 / 6.0 / 5.8 / 5.8 / 5.8, 4000 of 7813 groups
 // 49.6 / 38.2 / 34.2 / 32.2 / 30.8; 256 rows, 256 of 512 groups 13.2 / 21.1 / 35.5.
 uint32_t evict_parts(const cf_kv_evict_desc &d) {
@@ -478,7 +490,12 @@ uint32_t evict_parts(const cf_kv_evict_desc &d) {
 template <int D>
 void launch_evict(const cf_kv_evict_desc &d, bool tokens_here, hipStream_t s) {
   const dim3 grid(d.kv_head_count, d.seq_count, evict_parts(d));
-  if (d.max_groups / d.unit_groups <= 256) evict_kernel<D, 256><<<grid, 256, 0, s>>>(d, tokens_here);
+  // us with 256 / 512 / 1024 threads: 8 rows, 64 of 128 groups 5.7 / 6.1 / 7.2, 256 rows, 128 of 256 8.9 / 8.7 / 9.5, 256
+  // of 512 14.0 / 12.4 / 13.5, 512 of 1024 22.5 / 20.1 / 18.9; 512 rows, 512 of 1024 37.9 / 34.4 / 41.0
+  const uint32_t units = (d.max_groups + d.unit_groups - 1) / d.unit_groups;
+  const bool many = static_cast<uint64_t>(d.seq_count) * d.kv_head_count > cfd::cu_count();
+  if (units <= 256) evict_kernel<D, 256><<<grid, 256, 0, s>>>(d, tokens_here);
+  else if (units <= 512 || many) evict_kernel<D, 512><<<grid, 512, 0, s>>>(d, tokens_here);
   else evict_kernel<D, 1024><<<grid, 1024, 0, s>>>(d, tokens_here);
 }
 

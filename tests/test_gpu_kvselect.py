@@ -209,6 +209,23 @@ def test_select_long(dev, M, unit, S):
         assert np.array_equal(got, R.select_ref(q, codes, scales, t, pos, 4, unit, k, 1, 3)), k
 
 
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("S, H, M, unit, k", [(9, 29, 200, 1, 17),   # more rows than CUs, short: 256 threads a row
+                                              (9, 29, 300, 2, 30),   # more rows than CUs: 512
+                                              (9, 8, 1100, 1, 101),  # longer rows: 1024
+                                              (9, 8, 2200, 2, 300), (9, 29, 4100, 1, 64),  # more units than 512 threads take
+                                              (9, 1, 1030, 1, 64)])  # few rows: two launches at D = 128
+def test_select_workgroup_sizes(dev, D, S, H, M, unit, k):
+    rng = np.random.default_rng(M + D)
+    codes, scales = _records(rng, S, H, M, D)
+    codes[4, :, 50:], scales[4, :, 50:] = 127, np.inf  # records behind a row's length would rank first
+    q = rng.standard_normal((S, 2 * H, D)).astype(np.float32)
+    t = [64 * M, 0, 1, 64 * M - 65, 64 * 50, 64 * k + 1, 64 * (M // 2) - 3, 64 * M - 1, 64 * 129]
+    pos = [max(0, x - 1) for x in t]
+    got = _select(dev, codes, scales, q, t, pos, unit, k, 1, 2)
+    assert np.array_equal(got, R.select_ref(q, codes, scales, t, pos, 2, unit, k, 1, 2))
+
+
 # ---------------------------------------------------------------------------------------------------- attention
 class Case:
     """An INT8 (or rANS) cache of given lengths, its dequantised K and V in 64 bits, queries and positions."""
@@ -602,6 +619,14 @@ def test_evict_long(dev):
     _evict(dev, x, [64 * 20000 - 5], 1, 12345, 10, 100, 64, True)
     _evict(dev, x, [64 * 20000 - 5], 1, 12345, 10, 100, 64, False)
     _evict(dev, x, [64 * 20000 - 5], 2, 5001, 10, 100, 64, False)
+
+
+@pytest.mark.parametrize("place", [False, True])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("H, M, unit, budget", [(2, 500, 1, 301), (2, 1000, 2, 120), (65, 260, 1, 100), (65, 1030, 2, 99)])
+def test_evict_workgroup_sizes(dev, place, D, H, M, unit, budget):
+    x = _tables(np.random.default_rng(M + H), 4, H, M, D)
+    _evict(dev, x, [64 * M, 64 * M - 70, 64 * (budget * unit + 1) - 3, 640], unit, budget, 2, 5, D, place)
 
 
 @pytest.mark.parametrize("place", ["offsets", "tokens", "weights", "records"])
