@@ -9,6 +9,7 @@ u32 arrays are int32 tensors of the same bits; -1 is CF_KV_NO_UNIT. The *_desc f
 repeated calls (and as long as a graph captured with it); it holds the tensors it points at."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from dataclasses import dataclass
 
@@ -92,6 +93,22 @@ def _on_device(device: torch.device, fn, *args):
         return fn(*args)
 
 
+@contextlib.contextmanager
+def _working_on(stream, device: torch.device, *inputs: torch.Tensor):
+    """Makes `stream` (None: no change) the current one, behind what the current one has been given, so that tensors made
+    here are filled and let go of in the order of the work on it; the inputs' memory is kept for it."""
+    if stream is not None and stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+    if stream is None or stream == torch.cuda.current_stream(device):
+        yield
+        return
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        for t in inputs:
+            t.record_stream(stream)
+        yield
+
+
 def _with_workspace(desc, need: int, device: torch.device, stream) -> None:
     """Gives the descriptor a workspace for calls on `stream`, allocated for that stream."""
     if need:
@@ -149,17 +166,18 @@ def key_bounds(keys: torch.Tensor, first_page: torch.Tensor, page_counts: torch.
 
 def bounds_of(keys: torch.Tensor, stream=None) -> KeyBounds:
     """Bounds of dense keys [seq_count, kv_heads, T, D] (T a multiple of 16), group for group what kv.seal_device makes of
-    them."""
+    them. Made on `stream` (default: the current one) behind what the current stream has been given so far."""
     S, H, T, D = keys.shape
     if T % kv.PAGE_TOKENS:
         raise ValueError("T must be a multiple of 16, as for kv.seal_device")
     dev, pages = keys.device, T // kv.PAGE_TOKENS
     groups = -(-pages // kv.GROUP_PAGES)
-    out = empty_bounds(S, H, groups, D, dev)
-    g = torch.arange(S * H * groups, device=dev)
-    first = (g // groups) * pages + (g % groups) * kv.GROUP_PAGES
-    counts = torch.clamp(pages - (g % groups) * kv.GROUP_PAGES, max=kv.GROUP_PAGES).to(torch.int32)
-    return key_bounds(keys.reshape(-1, kv.PAGE_TOKENS, D), first, counts, out, stream=stream)
+    with _working_on(stream, dev, keys):
+        out = empty_bounds(S, H, groups, D, dev)
+        g = torch.arange(S * H * groups, device=dev)
+        first = (g // groups) * pages + (g % groups) * kv.GROUP_PAGES
+        counts = torch.clamp(pages - (g % groups) * kv.GROUP_PAGES, max=kv.GROUP_PAGES).to(torch.int32)
+        return key_bounds(keys.reshape(-1, kv.PAGE_TOKENS, D), first, counts, out, stream=stream)
 
 
 # ---------------------------------------------------------------------------------------------------- selection
