@@ -11,6 +11,7 @@ Every launch goes through libchromofold.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from dataclasses import dataclass, field
 
@@ -127,11 +128,12 @@ def encode_groups_device(codec: int, keys: torch.Tensor, values: torch.Tensor, h
     ws_bytes = int(L.cf_kv_encode_groups_workspace_bytes(codec, head_dim, n, tcount))
     if ws_bytes == 0:
         raise A.CfError(A.CF_ERR_INVALID_ARGUMENT, "cf_kv_encode_groups_workspace_bytes")
-    if workspace is None or workspace.numel() < ws_bytes:
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=pool.device)
-    offs = torch.empty(n, dtype=torch.int32, device=pool.device)
-    end = torch.zeros(1, dtype=torch.int64, device=pool.device)
-    status = torch.full((1,), -1, dtype=torch.int32, device=pool.device)
+    with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():  # filled on the stream of the call
+        if workspace is None or workspace.numel() < ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=pool.device)
+        offs = torch.empty(n, dtype=torch.int32, device=pool.device)
+        end = torch.zeros(1, dtype=torch.int64, device=pool.device)
+        status = torch.full((1,), -1, dtype=torch.int32, device=pool.device)
     s = (stream if stream is not None else torch.cuda.current_stream()).cuda_stream
     st = L.cf_kv_encode_groups_async(codec, keys.data_ptr(), values.data_ptr(), n, first_page.data_ptr(),
                                      page_counts.data_ptr(), _dptr(token_counts), head_dim, _dptr(tables), tcount,
@@ -236,7 +238,8 @@ def seal_device(codec: int, keys: torch.Tensor, values: torch.Tensor, tables: to
                 stream=None) -> BatchedKv:
     """Seal dense device K/V [seq_count, kv_heads, T, D] fp32 (T a multiple of 16, every sequence T tokens long)
     into a device pool with cf_kv_encode_groups_async, without a host round trip of the values. Group g of
-    (sequence s, head h) holds pages 4g..4g+3 of that (s, h). Synchronises once to read the pool end and status."""
+    (sequence s, head h) holds pages 4g..4g+3 of that (s, h). The groups are encoded on `stream` (default: the current
+    one) behind what the current stream has been given. Synchronises once to read the pool end and status."""
     S, H, T, D = keys.shape
     assert values.shape == keys.shape and T % PAGE_TOKENS == 0 and keys.is_contiguous() and values.is_contiguous()
     dev = keys.device
@@ -250,8 +253,14 @@ def seal_device(codec: int, keys: torch.Tensor, values: torch.Tensor, tables: to
     cont = (gl % 2 == 1).to(torch.uint8)  # groups 2k, 2k + 1 of each (sequence, head) form one chain
     cap = int(A.lib().cf_kv_group_blob_max_bytes(codec, D)) * S * H * ngr
     pool = torch.empty(cap, dtype=torch.uint8, device=dev)
+    here = torch.cuda.current_stream(dev) if stream is not None else None
+    if here is not None:
+        stream.wait_stream(here)  # for the arrays made above and the pool's memory
     r = encode_groups_device(codec, keys.view(-1, PAGE_TOKENS, D), values.view(-1, PAGE_TOKENS, D), D, tables, first,
                              counts, pool, 0, heads, None, None, stream, continues=cont)
+    if here is not None:
+        here.wait_stream(stream)  # for what is read below, and before the arrays above are let go of
+        r.offsets.record_stream(here)
     st, end = int(r.status.item()), int(r.pool_end.item())
     if st != 0:
         raise A.CfError(st, "cf_kv_encode_groups_async (device status)")

@@ -26,3 +26,24 @@ def test_bounds_of_on_another_stream(dev):
         del keys
         side.synchronize()
         assert np.array_equal(down(b.scales).ravel(), scales) and np.array_equal(down(b.codes).reshape(codes.shape), codes)
+
+
+def test_seal_device_on_another_stream(dev):
+    import torch
+    from chromofold_amd import kv
+    rng = np.random.default_rng(2)
+    k, v = (rng.standard_normal((2, 3, 208, 64)).astype(np.float32) for _ in range(2))
+    tables = np.concatenate([kv.build_table(x[0, h].reshape(-1, 16, 64)) for h in range(3) for x in (k, v)])
+    want = kv.seal_device(kv.CODEC_RANS_HYBRID, up(dev, k), up(dev, v), up(dev, tables))
+    q, pos = up(dev, rng.standard_normal((2, 6, 64)).astype(np.float32)), up(dev, np.array([207, 100], np.uint32))
+    ref, out = torch.empty_like(q), torch.empty_like(q)
+    want.attention(q, ref, pos, 0.125)
+    host, side = (up(dev, k), up(dev, v)), torch.cuda.Stream(dev)
+    for _ in range(3):
+        busy = torch.ones(4096, 4096, device=dev)
+        for _ in range(4):
+            busy = busy @ busy * 1e-4
+        got = kv.seal_device(kv.CODEC_RANS_HYBRID, host[0] * 1.0, host[1] * 1.0, up(dev, tables), stream=side)
+        assert torch.equal(got.group_offsets, want.group_offsets) and got.pool.numel() == want.pool.numel()
+        got.attention(q, out, pos, 0.125)
+        assert torch.equal(out, ref)
