@@ -273,7 +273,8 @@ struct Spread {
 template <int D, int GT>
 struct RowState {
   float m[4], l[4];
-  int e;  // acc holds sums in units of 2^e
+  int e;    // acc holds sums in units of 2^e
+  int top;  // and they are below 2^(top + 54); see kDrop
   float4_t acc[D / 16];
   float unit[4];  // log2-unit factor of the heads' scores, without the page's scale
   half8_t qh[D / 32], ql[D / 32];
@@ -282,7 +283,7 @@ struct RowState {
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int r = 0; r < 4; ++r) m[r] = -INFINITY, l[r] = 0.0f;
-    e = -(1 << 20);
+    e = top = -(1 << 20);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) acc[i] = float4_t{0, 0, 0, 0};
     bad = false;
@@ -359,23 +360,49 @@ struct RowState {
     for (int r = 0; r < 4; ++r) moved |= mx[r] > m[r];
     // units of the P.V sums: the exponent of the group's largest V scale among its visible pages, less 15, so that
     // weights p vs lie in [0, 2^15) and those down to 2^-29 of that are normal f16 numbers. Sums move to a larger unit
-    // at once and to a smaller one when 2^8 below (a factor of a power of two; clamped so that it cannot overflow).
-    constexpr int kNone = -(1 << 24);
+    // at once (a factor of a power of two) and to a smaller one when 2^8 below: then weights down to 2^-21 of the group's
+    // largest are normal.
+    // 2^31 tokens of weights below 2^15 and symbols up to 2^7 add up to less than 2^53 of the largest unit so far, `top`: in
+    // a unit down to 2^-kDrop of it they stay finite. For a smaller one, the sums as they are say how far it may fall.
+    constexpr int kNone = -(1 << 24), kSum = 53, kDrop = 60;
     const int ep = page_vis ? __builtin_amdgcn_frexp_expf(vs) - 15 : kNone;
     const int eb = max(max(__builtin_amdgcn_readlane(ep, 0), __builtin_amdgcn_readlane(ep, 4)),
                        max(__builtin_amdgcn_readlane(ep, 8), __builtin_amdgcn_readlane(ep, 12)));
     int e_new = e;
-    if (eb != kNone && (eb > e || eb < e - 8)) e_new = max(eb, e - 60);
+    if (eb != kNone && (eb > e || eb < e - 8)) e_new = eb;
+    top = max(top, e_new);
     if (__builtin_amdgcn_ballot_w64(moved) || e_new != e) {
+      float f[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float mn = fmaxf(m[r], mx[r]);
-        const float al = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - mn);
+        f[r] = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - mn);  // 0 before the first visible token
         m[r] = mn;
-        l[r] *= al;
-        const float f = ldexpf(al, max(e - e_new, -200));  // 0 before the first visible token
+        l[r] *= f[r];
+      }
+      if (e_new < top - kDrop) {
+        float big = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) acc[i][r] *= f;
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            acc[i][r] *= f[r];
+            if (static_cast<uint32_t>(4 * b + r) < gqa) big = fmaxf(big, fabsf(acc[i][r]));  // (other rows hold anything)
+          }
+        big = cfd::rows4_max(cfd::row16_max(big));
+        top = big > 0.0f ? max(e_new, __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(big)) + e - kSum) : e_new;
+        e_new = max(e_new, top - kDrop);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) acc[i][r] = ldexpf(acc[i][r], e - e_new);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f[r] = ldexpf(f[r], max(e - e_new, -200));
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) acc[i][r] *= f[r];
+        }
       }
       e = e_new;
     }

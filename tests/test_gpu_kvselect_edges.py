@@ -4,7 +4,9 @@ import numpy as np
 import pytest
 
 import kvselect_helpers as R
-from test_gpu_kvselect import dev, down, u32, up  # noqa: F401 (dev: the fixture)
+import test_gpu_kvselect as T
+from kv_helpers import make_seqs
+from test_gpu_kvselect import dev, down, up  # noqa: F401 (dev: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +49,85 @@ def test_seal_device_on_another_stream(dev):
         assert torch.equal(got.group_offsets, want.group_offsets) and got.pool.numel() == want.pool.numel()
         got.attention(q, out, pos, 0.125)
         assert torch.equal(out, ref)
+
+
+# ---------------------------------------------------------------------------------------------------- V scales
+def cache(monkeypatch, dev, lens, H, gqa, D, seed, codec=1, edit=None, **how):
+    """A Case whose data `edit(data)` may change before it is sealed (coded pools as chain pairs)."""
+    def seqs(*args, **kw):
+        data = make_seqs(*args, **kw)
+        if edit:
+            edit(data)
+        return data
+    monkeypatch.setattr(T, "make_seqs", seqs)
+    return T.Case(dev, lens, H, gqa, D, seed, codec=codec, **how)
+
+
+def set_v_scales(c, s, h, g, scales):
+    """Writes the V scales of the pages of group g into its header (64-byte header: fp32 x 4 at 48), and the reference's."""
+    o = 16 * int(c.kvb.host_offsets[s, h, g])
+    old = down(c.kvb.pool[o + 48: o + 64]).view(np.float32)
+    new = np.array(scales, np.float32)
+    c.kvb.pool[o + 48: o + 64] = up(c.dev, new.view(np.uint8))
+    for p in range(4):
+        t = slice(64 * g + 16 * p, 64 * g + 16 * p + 16)
+        c.v[s][h][t] *= float(new[p]) / float(old[p])
+
+
+def attend(c, call, splits):
+    """The rows' results from the call that can select groups, or from the batched one."""
+    import torch
+    if call == "selected":
+        return c.run(splits=splits)[0]
+    out = torch.full(c.q.shape, float("nan"), device=c.dev)
+    c.kvb.attention(up(c.dev, c.q), out, up(c.dev, np.array(c.pos, np.uint32)), c.scale, splits=splits)
+    return down(out).astype(np.float64)
+
+
+CALLS = [(1, "selected", 1), (1, "selected", 4), (1, "selected", 8), (1, "selected", 16)]
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("codec, call, gqa", CALLS)
+def test_v_scales_that_fall_in_steps(dev, monkeypatch, codec, call, gqa, D):
+    """V scales down from 2^30 to 2^-110 in steps of less than 2^60, again and again in each wavefront's groups: sums of the
+    large ones stay finite, whatever unit the small ones ask for, and what a later group brings back up is not lost."""
+    steps = [30, -25, -80, -110, -110]
+    c = cache(monkeypatch, dev, [64 * 40, 64 * 40 - 7], 1, gqa, D, 201, codec)
+    for s in range(2):
+        for g in range(40):
+            set_v_scales(c, s, 0, g, [2.0 ** steps[g % 5]] * 4)
+    o, _, mag, big, low = R.attend_ref(c.q, c.k, c.v, c.lens, c.pos, gqa, c.scale, None, 1, c.M)
+    tol = R.tolerance(big, D)[..., None] * mag + 2.0 ** -23 * np.abs(o) + low
+    for splits in (1, 2):
+        out = attend(c, call, splits)
+        assert np.isfinite(out).all(), splits
+        assert (np.abs(out - o) <= tol).all(), splits
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("codec, call, gqa", CALLS)
+def test_small_v_behind_large_v_of_no_weight(dev, monkeypatch, codec, call, gqa, D):
+    """Each wavefront's first groups have V scales of 2^20, 2^-30 and 2^-60 and scores so low (150 below the others', in log2
+    units 200 or more) that the rest, with V scales of 2^-95 and less, are all of the output: they are held in units that
+    follow them, not the sums that have faded."""
+    exps = [20, -30, -60, -95, -100, -95, -101, -95, -97, -99]
+    n = len(exps)
+    away = np.array([g % n < 3 for g in range(4 * n)])
+
+    def edit(data):
+        for k, _ in data:
+            k *= np.float32(0.02)
+            k[..., 0] = np.where(np.repeat(away, 64), -8.0, 8.0)
+    c = cache(monkeypatch, dev, [64 * 4 * n], 1, gqa, D, 202, codec, edit)
+    for g in range(4 * n):
+        set_v_scales(c, 0, 0, g, [2.0 ** exps[g % n]] * 4)
+    c.q[:, :, 0], c.scale = 1.0, 10.0
+    o, _, mag, big, _ = R.attend_ref(c.q, c.k, c.v, c.lens, c.pos, gqa, c.scale, None, 1, c.M)
+    # weights of the groups with V scales of 2^-95 may be held in units up to 8 binades above their own: 2^-25 of a unit
+    # 2^(-95 + 1 - 15 + 8) each, times a symbol, over a sum of weights that is at least 1
+    floor = 2.0 ** (-25 - 95 + 1 - 15 + 8) * 128 * c.lens[0]
+    for splits in (1, 2):
+        out = attend(c, call, splits)
+        assert (np.abs(out - o) <= R.tolerance(big, D)[..., None] * mag + 2.0 ** -23 * np.abs(o) + floor).all(), splits
+        assert (np.abs(o) > 2 * floor).mean() > 0.9
