@@ -260,7 +260,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * W) void kv_batched_kernel(cf_kv_batc
   const uint32_t *grow = d.group_offsets + (static_cast<size_t>(seq) * d.kv_head_count + head) * d.max_groups;
 
   float m_run[kGqa], l_run[kGqa];
-  int e_run = -(1 << 20);  // exponent of the wavefront's P.V units (set by its first group; see group_body)
+  cfkv::VUnit<RANS> unit;  // of the wavefront's P.V sums (see group_body)
   float4_t acc_v[D / 16];
 #pragma unroll
   for (int h = 0; h < kGqa; ++h) {
@@ -383,12 +383,12 @@ __global__ CF_KV_OCC __launch_bounds__(64 * W) void kv_batched_kernel(cf_kv_batc
     if (RANS && gcodec == CF_KV_CODEC_RANS_HYBRID) {
       group_body<D, CF_KV_CODEC_RANS_HYBRID, KL>(stage_next, pre, nlw, st, raw_of(cur, chain),
                                                  reinterpret_cast<const uint16_t *>(buf), cnt, s_tab, qhi, qlo, qsum,
-                                                 s_p[wave], vl, lane, tok_ok, ks, vs, e_run, m_run, l_run, acc_v);
+                                                 s_p[wave], vl, lane, tok_ok, ks, vs, unit, gqa, m_run, l_run, acc_v);
     } else {  // raw int8 group (the INT8 codec, or the raw fallback of a group holding -128)
       // an INT8-codec launch streams its groups; raw groups inside a RANS launch (e.g. a shared prefix) are cached
       group_body<D, CF_KV_CODEC_INT8, KL, const uint16_t *, decltype(stage_next), false, false, !RANS>(
           stage_next, pre, nlw, st, reinterpret_cast<const uint32_t *>(cur + kHdr), static_cast<const uint16_t *>(nullptr),
-          0, s_tab, qhi, qlo, qsum, s_p[wave], vl, lane, tok_ok, ks, vs, e_run, m_run, l_run, acc_v);
+          0, s_tab, qhi, qlo, qsum, s_p[wave], vl, lane, tok_ok, ks, vs, unit, gqa, m_run, l_run, acc_v);
     }
     prev = gi;
     gi = gn;
@@ -418,7 +418,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * W) void kv_batched_kernel(cf_kv_batc
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
     for (int h = 0; h < kGqa; ++h) {
-      float v = G < 2 ? ldexpf(acc_v[i][h], e_run) : 0.0f;
+      float v = G < 2 ? ldexpf(acc_v[i][h], unit.e()) : 0.0f;
       v += __shfl_xor(v, 16);
       v += __shfl_xor(v, 32);
       acc_v[i][h] = v;
@@ -663,10 +663,10 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesWide) void kv_span_kernel(cf_k
   };
 
   float m_run[kGqa], l_run[kGqa];
-  int e_run;
+  cfkv::VUnit<RANS> unit;
   float4_t acc_v[D / 16];
   auto reset = [&]() {
-    e_run = -(1 << 20);
+    unit = {};
 #pragma unroll
     for (int h = 0; h < kGqa; ++h) {
       m_run[h] = -INFINITY;
@@ -779,11 +779,11 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesWide) void kv_span_kernel(cf_k
     if (RANS && gcodec == CF_KV_CODEC_RANS_HYBRID) {
       group_body<D, CF_KV_CODEC_RANS_HYBRID, KL>(stage_next, pre, nlw, st, raw_of(curb, chain),
                                                  reinterpret_cast<const uint16_t *>(buf), cnt, s_tab, qhi, qlo, qsum,
-                                                 s_p[wave], vl, lane, tok_ok, ks, vs, e_run, m_run, l_run, acc_v);
+                                                 s_p[wave], vl, lane, tok_ok, ks, vs, unit, gqa, m_run, l_run, acc_v);
     } else {
       group_body<D, CF_KV_CODEC_INT8, KL, const uint16_t *, decltype(stage_next), false, false, !RANS>(
           stage_next, pre, nlw, st, reinterpret_cast<const uint32_t *>(curb + kHdr), static_cast<const uint16_t *>(nullptr),
-          0, s_tab, qhi, qlo, qsum, s_p[wave], vl, lane, tok_ok, ks, vs, e_run, m_run, l_run, acc_v);
+          0, s_tab, qhi, qlo, qsum, s_p[wave], vl, lane, tok_ok, ks, vs, unit, gqa, m_run, l_run, acc_v);
     }
     fresh = false;
     if (nc.s != cs && nc.s != kNoSeq) {
@@ -805,7 +805,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesWide) void kv_span_kernel(cf_k
         ag[i] = 0.0f;
 #pragma unroll
         for (int h = 0; h < kGqa; ++h) {
-          const float v = cfd::rows4_sum(G < 2 ? ldexpf(acc_v[i][h], e_run) : 0.0f);
+          const float v = cfd::rows4_sum(G < 2 ? ldexpf(acc_v[i][h], unit.e()) : 0.0f);
           ag[i] = G == h ? v : ag[i];
         }
       }
@@ -841,7 +841,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesWide) void kv_span_kernel(cf_k
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
       for (int h = 0; h < kGqa; ++h) {
-        const float v = cfd::rows4_sum(G < 2 ? ldexpf(acc_v[i][h], e_run) : 0.0f);
+        const float v = cfd::rows4_sum(G < 2 ? ldexpf(acc_v[i][h], unit.e()) : 0.0f);
         if (lane < 16) red[h * (D + 2) + t + 16 * i] = v;
       }
 #pragma unroll
@@ -1521,7 +1521,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesNarrow) void seam_group_kernel
   const uint32_t qtok = d.query_token_begin;
   const uint32_t wlo = (d.causal_window == 0 || qtok + 1 <= d.causal_window) ? 0u : qtok + 1 - d.causal_window;
   float m_run[kGqa], l_run[kGqa];
-  int e_run = -(1 << 20);
+  cfkv::VUnit<true> unit;
   float4_t acc_v[D / 16];
 #pragma unroll
   for (int h = 0; h < kGqa; ++h) {
@@ -1659,7 +1659,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesNarrow) void seam_group_kernel
         uint32_t ends[2];
         group_body<D, CF_KV_CODEC_RANS_HYBRID, 0, const uint16_t *, decltype(stage_next), true, true>(
             stage_next, pre, nlw, st, raw_of(cur), reinterpret_cast<const uint16_t *>(buf), cur.cnt, s_tab, qhi, qlo,
-            qsum, s_p[wave], nullptr, lane, tok_ok, cur.ks, cur.vs, e_run, m_run, l_run, acc_v, ends, page_vis);
+            qsum, s_p[wave], nullptr, lane, tok_ok, cur.ks, cur.vs, unit, gqa, m_run, l_run, acc_v, ends, page_vis);
         // a group coded on its own ends where the encoder started (2^16 in every lane) and consumed exactly its words
         const uint32_t nk = cur.cnt & 0xFFFFu, nv = cur.cnt >> 16;
         const bool ok = st[0] == 65536u && st[1] == 65536u && ends[0] == nk && ends[1] == nk + nv;
@@ -1668,7 +1668,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesNarrow) void seam_group_kernel
         group_body<D, CF_KV_CODEC_INT8, 0, const uint16_t *, decltype(stage_next), false, true>(
             stage_next, pre, nlw, st, reinterpret_cast<const uint32_t *>(cur.blob + kHdr),
             static_cast<const uint16_t *>(nullptr), 0, s_tab, qhi, qlo, qsum, s_p[wave], nullptr, lane, tok_ok,
-            cur.ks, cur.vs, e_run, m_run, l_run, acc_v, nullptr, page_vis);
+            cur.ks, cur.vs, unit, gqa, m_run, l_run, acc_v, nullptr, page_vis);
       }
     }
     cur = nx;
@@ -1683,7 +1683,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesNarrow) void seam_group_kernel
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
     for (int h = 0; h < kGqa; ++h) {
-      float v = G < 2 ? ldexpf(acc_v[i][h], e_run) : 0.0f;
+      float v = G < 2 ? ldexpf(acc_v[i][h], unit.e()) : 0.0f;
       v += __shfl_xor(v, 16);
       v += __shfl_xor(v, 32);
       acc_v[i][h] = v;

@@ -94,7 +94,26 @@ __device__ __forceinline__ void wave64_max4(float (&x)[4]) {
   for (int h = 0; h < 4; ++h) x[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x[h]), 63));
 }
 
-// Decode one page group (K scores, softmax, V accumulation).
+// Units of a wavefront's P.V sums: acc holds them in units of 2^e, and they are below 2^(top + 54); see kDrop. CODED launches
+// keep both in one register and settle `top` at the start of a group, others in two and at its end: these kernels' steps
+// overlap as far as their registers go, and a register or a branch more elsewhere costs 2-4 % (256 sequences behind a shared
+// prefix 156.5 us, 160-163 the other way; INT8 hd 64 17.3, 17.8 the other way).
+template <bool CODED>
+struct VUnit {
+  int e_ = -(1 << 20), top_ = -(1 << 20);
+  __device__ __forceinline__ int e() const { return e_; }
+  __device__ __forceinline__ int top() const { return top_; }
+  __device__ __forceinline__ void set(int e, int top) { e_ = e, top_ = top; }
+};
+template <>
+struct VUnit<true> {
+  int both = -(1 << 14) * 65537;
+  __device__ __forceinline__ int e() const { return static_cast<int16_t>(both); }
+  __device__ __forceinline__ int top() const { return both >> 16; }
+  __device__ __forceinline__ void set(int e, int top) { both = (top << 16) | (e & 0xFFFF); }
+};
+
+// Decode one page group (K scores, softmax, V accumulation) for `heads` query heads (the other rows hold anything).
 // RANS groups: `st` holds the chain's lane states on entry (K, V) and the states the group ends with on return;
 // the word streams are read through `wk` (the wave's LDS staging buffer, K stream then V); `raw` points at the
 // group's raw words. `pre` holds 14 raw words (7 K + 7 V): on entry the group's first sign group, on return the
@@ -113,18 +132,34 @@ __device__ __forceinline__ void wave64_max4(float (&x)[4]) {
 // groups' words are read with non-temporal loads (for launches whose groups are each read once). p_out, if given, receives
 // the lane's token's weights exp(score - m_run) of the heads.
 template <int D, int CODEC, int KL, typename WordPtr, typename Hook, bool kEnds = false, bool kPageVis = false,
-          bool kStreamRaw = false>
+          bool kStreamRaw = false, bool kCoded>
 __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&pre)[14], const uint32_t *nlw,
                                            uint32_t (&st)[2], const uint32_t *__restrict__ raw, WordPtr wk,
                                            uint32_t cnt_kv, const uint2 (*__restrict__ s_tab)[kSlots],
                                            const half4_t *qhi, const half4_t *qlo, const float *qsum,
                                            _Float16 (*s_pw)[4][kGqa][16], uint32_t *__restrict__ vl, int lane,
-                                           bool tok_ok, float ks, float vs, int &e_run, float *m_run, float *l_run,
-                                           float4_t *acc_v, uint32_t *ends = nullptr, bool page_vis = false,
+                                           bool tok_ok, float ks, float vs, VUnit<kCoded> &unit, uint32_t heads, float *m_run,
+                                           float *l_run, float4_t *acc_v, uint32_t *ends = nullptr, bool page_vis = false,
                                            float *p_out = nullptr) {
   constexpr int NQ = D / 4, RAW = raw_words<D>();
   constexpr bool RANS = CODEC == CF_KV_CODEC_RANS_HYBRID;
   const int G = lane >> 4, t = lane & 15;
+  // Where the units of the P.V sums have fallen, the sums as they are say how far they may fall from here: at least by 2^60,
+  // unless sums that large are still in them.
+  constexpr int kSum = 53, kDrop = 72;
+  auto settle = [&] {
+    if (unit.top() <= unit.e() + kDrop - 60) return;
+    float big = 0.0f;
+#pragma unroll
+    for (int h = 0; h < kGqa; ++h)
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        if (static_cast<uint32_t>(h) < heads) big = fmaxf(big, fabsf(acc_v[i][h]));
+    big = cfd::rows4_max(cfd::row16_max(big));
+    const int e = unit.e(), x = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(big));
+    unit.set(e, big > 0.0f ? max(e, x + e - kSum) : e);
+  };
+  if constexpr (kCoded) settle();
   float4_t sa = {0, 0, 0, 0}, sb = {0, 0, 0, 0};
   uint32_t vb[NQ];                         // V: magnitude bytes (RANS) or offset-binary symbols (INT8) per quad
   auto put_v = [&](auto qc, uint32_t v) {
@@ -240,23 +275,23 @@ __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&
   // P.V runs on v_mfma_f32_16x16x32_f16 with k = 8 tokens of each of the 4 pages (page G's from lane group G), so
   // one MFMA sums all four pages: rows 0-3 are the 4 heads' hi parts of the weights p * v_scale, rows 4-7 their lo
   // parts (rows 8-15 repeat rows 0-7 and are dropped), 16 dims per MFMA. The lane's accumulators acc_v hold rows
-  // 4G..4G+3: the hi (G = 0) or lo (G = 1) sums. The wavefront keeps them in units of 2^e_run with e = (exponent of
+  // 4G..4G+3: the hi (G = 0) or lo (G = 1) sums. The wavefront keeps them in units of 2^e with e = (exponent of
   // the group's largest V scale among its pages with a visible token) - 15 (+ 24 for RANS groups, whose V operands
   // are q * 2^-24): every f16 weight lies in [0, 2^15) whatever the V magnitude, weights down to 2^-29 of the
   // running maximum stay normal f16 numbers (a row whose heaviest tokens have V = 0 is carried by such small
   // weights), and hi + lo keep ~22 bits for every page within 2^18 of the group's largest V scale (the lo part of a
   // page further below loses bits gradually: ~16 bits at 2^24, those of one f16 at 2^29). Moving to new units is an
-  // exact power-of-two factor folded into the softmax rescale; a drop of more than 2^60 is clamped so that the
-  // rescale cannot overflow.
+  // exact power-of-two factor folded into the softmax rescale. 2^31 tokens of weights below 2^15 and values up to 2^7
+  // add up to less than 2^53 of the largest unit so far (unit.top()): in a unit down to 2^-kDrop of it they stay finite.
   constexpr int kOpExp = RANS ? 24 : 0;
   constexpr int kNone = -(1 << 24);
   // tokens are visible as a prefix of each page, so a page's lane 16 G is visible iff any of its tokens is
   const int ep = (kPageVis ? page_vis : tok_ok) ? __builtin_amdgcn_frexp_expf(vs) - 15 + kOpExp : kNone;
   const int eb = max(max(__builtin_amdgcn_readlane(ep, 0), __builtin_amdgcn_readlane(ep, 16)),
                      max(__builtin_amdgcn_readlane(ep, 32), __builtin_amdgcn_readlane(ep, 48)));
-  const int nb = eb != kNone ? max(eb, e_run - 60) : e_run;
-  const int de = e_run - nb;
-  e_run = nb;
+  const int nb = eb != kNone ? max(eb, unit.top() - kDrop) : unit.e();
+  const int de = unit.e() - nb;
+  unit.set(nb, max(unit.top(), nb));
   const float vsn = ldexpf(vs, kOpExp - nb);
   float alpha[kGqa], pr[kGqa];
 #pragma unroll
@@ -321,6 +356,7 @@ __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  if constexpr (!kCoded) settle();
 }
 
 }  // namespace cfkv

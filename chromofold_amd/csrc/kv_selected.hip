@@ -858,7 +858,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
   __syncthreads();  // s_q is dead from here on
 
   float m_run[kGqa], l_run[kGqa];
-  int e_run = -(1 << 20);
+  VUnit<true> unit;
   cfkv::float4_t acc_v[D / 16];
 #pragma unroll
   for (int h = 0; h < kGqa; ++h) m_run[h] = -INFINITY, l_run[h] = 0.0f;
@@ -960,13 +960,13 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
         if (gcodec == CF_KV_CODEC_RANS_HYBRID)
           group_body<D, CF_KV_CODEC_RANS_HYBRID, 0>(stage_next, pre, nlw, st, raw_of(here_blob, chain),
                                                     reinterpret_cast<const uint16_t *>(buf), cnt, s_tab, qhi, qlo, qsum, s_p[wave],
-                                                    static_cast<uint32_t *>(nullptr), lane, tok_ok, ks, vs, e_run, m_run, l_run,
+                                                    static_cast<uint32_t *>(nullptr), lane, tok_ok, ks, vs, unit, gqa, m_run, l_run,
                                                     acc_v, static_cast<uint32_t *>(nullptr), false, p);
         else
           group_body<D, CF_KV_CODEC_INT8, 0, const uint16_t *>(
               stage_next, pre, nlw, st, reinterpret_cast<const uint32_t *>(here_blob + cfkv::kHdr),
               static_cast<const uint16_t *>(nullptr), 0, s_tab, qhi, qlo, qsum, s_p[wave], static_cast<uint32_t *>(nullptr), lane,
-              tok_ok, ks, vs, e_run, m_run, l_run, acc_v, static_cast<uint32_t *>(nullptr), false, p);
+              tok_ok, ks, vs, unit, gqa, m_run, l_run, acc_v, static_cast<uint32_t *>(nullptr), false, p);
         if (stats) {
 #pragma unroll
           for (int h = 0; h < kGqa; ++h) {
@@ -991,7 +991,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
   for (int i = 0; i < D / 16; ++i)
 #pragma unroll
     for (int h = 0; h < kGqa; ++h) {
-      float v = G < 2 ? ldexpf(acc_v[i][h], e_run) : 0.0f;
+      float v = G < 2 ? ldexpf(acc_v[i][h], unit.e()) : 0.0f;
       v += __shfl_xor(v, 16);
       v += __shfl_xor(v, 32);
       acc_v[i][h] = v;

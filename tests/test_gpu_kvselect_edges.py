@@ -84,7 +84,8 @@ def attend(c, call, splits):
     return down(out).astype(np.float64)
 
 
-CALLS = [(1, "selected", 1), (1, "selected", 4), (1, "selected", 8), (1, "selected", 16)]
+CALLS = [(1, "selected", 1), (1, "selected", 4), (1, "selected", 8), (1, "selected", 16), (2, "selected", 1), (2, "selected", 4),
+         (1, "batched", 1), (1, "batched", 4), (2, "batched", 1), (2, "batched", 4)]
 
 
 @pytest.mark.parametrize("D", [128, 64])
@@ -106,11 +107,13 @@ def test_v_scales_that_fall_in_steps(dev, monkeypatch, codec, call, gqa, D):
 
 
 @pytest.mark.parametrize("D", [128, 64])
-@pytest.mark.parametrize("codec, call, gqa", CALLS)
+@pytest.mark.parametrize("codec, call, gqa", [c for c in CALLS if c[:2] != (1, "batched")])
 def test_small_v_behind_large_v_of_no_weight(dev, monkeypatch, codec, call, gqa, D):
     """Each wavefront's first groups have V scales of 2^20, 2^-30 and 2^-60 and scores so low (150 below the others', in log2
     units 200 or more) that the rest, with V scales of 2^-95 and less, are all of the output: they are held in units that
-    follow them, not the sums that have faded."""
+    follow them, not the sums that have faded. (Not for the batched call of an INT8 pool: its K operands are symbols + 1024,
+    whose sums over D / 4 instructions of each of two parts may be off by 2 D / 4 * 2^-24 * 1280 sum |x| of the queries x, here
+    0.3 in a score, so that no bound on its outputs would tell.)"""
     exps = [20, -30, -60, -95, -100, -95, -101, -95, -97, -99]
     n = len(exps)
     away = np.array([g % n < 3 for g in range(4 * n)])
