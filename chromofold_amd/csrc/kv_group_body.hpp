@@ -292,7 +292,9 @@ __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&
   const int nb = eb != kNone ? max(eb, unit.top() - kDrop) : unit.e();
   const int de = unit.e() - nb;
   unit.set(nb, max(unit.top(), nb));
-  const float vsn = ldexpf(vs, kOpExp - nb);
+  // 0 for a token that is not visible: its page's scale may be anything (that of an absent page is 1, which small units
+  // make infinite), and 0 * inf would be in every row's sum
+  const float vsn = tok_ok ? ldexpf(vs, kOpExp - nb) : 0.0f;
   float alpha[kGqa], pr[kGqa];
 #pragma unroll
   for (int h = 0; h < kGqa; ++h) {

@@ -134,3 +134,41 @@ def test_small_v_behind_large_v_of_no_weight(dev, monkeypatch, codec, call, gqa,
         out = attend(c, call, splits)
         assert (np.abs(out - o) <= R.tolerance(big, D)[..., None] * mag + 2.0 ** -23 * np.abs(o) + floor).all(), splits
         assert (np.abs(o) > 2 * floor).mean() > 0.9
+
+
+# ---------------------------------------------------------------------------------------------------- what is not visible
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("codec, call, gqa", CALLS)
+def test_scales_behind_the_query(dev, monkeypatch, codec, call, gqa, D):
+    """Pages of a row's last group that the query must not see, with V scales of infinity and NaN (as of a sealed page that
+    holds them) and K scales of NaN: outputs and weights as without them. Row 1: raw groups in a coded pool. Row 2: the last
+    page is cut, and its pages behind the query are absent."""
+    c = cache(monkeypatch, dev, [320, 320, 261], 2, gqa, D, 203, codec, pos=[269, 269, 260],
+              **({"raw_groups": {1: 5}} if codec == 2 else {}))
+    bad = np.array([np.nan, np.inf, -np.inf], np.float32)
+    for s in (0, 1):
+        for h in (0, 1):
+            o = 16 * int(c.kvb.host_offsets[s, h, 4])
+            c.kvb.pool[o + 52: o + 64] = up(dev, np.roll(bad, h).view(np.uint8))
+            c.kvb.pool[o + 36: o + 48] = up(dev, np.full(3, np.nan, np.float32).view(np.uint8))
+    ref = R.attend_ref(c.q, c.k, c.v, c.lens, c.pos, gqa, c.scale, None, 1, c.M)
+    o, w, mag, big, low = ref
+    for splits in (0, 1, 3):
+        out = attend(c, call, splits)
+        assert np.isfinite(out).all(), splits
+        if call == "selected":
+            c.compare(ref, *c.run(splits=splits))
+        else:  # the batched call's bar (its scores are not held as finely)
+            assert (np.abs(out - o).max(2) <= 1e-3 * np.abs(o).max(2)).all()
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("codec, call, gqa", CALLS)
+def test_small_v_beside_absent_pages(dev, monkeypatch, codec, call, gqa, D):
+    # V of 2^-112 and pages that are not there, whose scale of 1 is 2^128 in these units
+    c = cache(monkeypatch, dev, [69, 5, 300], 1, gqa, D, 204, codec, v_mult=[[2.0 ** -112]] * 3)
+    o, _, mag, big, low = R.attend_ref(c.q, c.k, c.v, c.lens, c.pos, gqa, c.scale, None, 1, c.M)
+    for splits in (0, 1):
+        out = attend(c, call, splits)
+        assert np.isfinite(out).all()
+        assert (np.abs(out - o).max(2) <= 1e-3 * np.abs(o).max(2)).all()
