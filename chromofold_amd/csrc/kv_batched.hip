@@ -1097,6 +1097,7 @@ __global__ __launch_bounds__(kPfxThreads) __attribute__((amdgpu_waves_per_eu(2))
   float m = -INFINITY;      // row j's softmax reference (same in its 4 lanes), at most ln 2 below the running maximum
   float l = 0.0f;           // the lane's share of row j's sum (its 4 lanes are added at the end)
   int e_run = -(1 << 20);   // acc is kept in units of 2^e_run (from the V-scale exponents of the groups)
+  int e_top = -(1 << 20);   // and holds sums below 2^(e_top + 55) (see below)
   bool coded = false;       // a prefix group that is not INT8 was met
   float4_t acc[D / 16];     // O[rows 4kg + r][dims 16 dt + j]
 #pragma unroll
@@ -1196,15 +1197,33 @@ __global__ __launch_bounds__(kPfxThreads) __attribute__((amdgpu_waves_per_eu(2))
       const float alpha = m == -INFINITY ? 0.0f : __expf(m - mn);
       m = mn;
       l *= alpha;
-      // moving to the group's units is an exact power of two (a drop of more than 2^60 is clamped)
-      const int en = max(ev, e_run - 60), de = e_run - en;
+      // moving to the group's units is an exact power of two. 2^31 tokens of weights below 2^16 and values up to 2^7 add up
+      // to less than 2^54 of the largest unit so far, e_top: in units down to 2^-kDrop of it they stay finite. Where the
+      // units have fallen, the sums as they are say how far they may fall the next time: by 2^60, unless sums that large
+      // are still in them.
+      constexpr int kSum = 54, kDrop = 72;
+      const int en = max(ev, e_top - kDrop), de = e_run - en;
       e_run = en;
+      e_top = max(e_top, en);
       // O's rows are 4kg + r, whose alpha lives in lane 4kg + r
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float ar = ldexpf(__shfl(alpha, 4 * kg + r), de);
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) acc[dt][r] *= ar;
+      }
+      if (e_top > e_run + kDrop - 60) {
+        float big = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool real = tile * 16 + wave * 4 + (4 * kg + r) / 4 < d.seq_count && (4 * kg + r) % 4 < gqa;
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt)
+            if (real) big = fmaxf(big, fabsf(acc[dt][r]));
+        }
+        big = cfd::rows4_max(cfd::row16_max(big));
+        const int x = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(big));
+        e_top = big > 0.0f ? max(e_run, x + e_run - kSum) : e_run;
       }
     }
     // P V over page pairs (2s, 2s + 1); the weights p * v_scale as f16 hi + lo parts

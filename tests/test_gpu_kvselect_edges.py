@@ -172,3 +172,68 @@ def test_small_v_beside_absent_pages(dev, monkeypatch, codec, call, gqa, D):
         out = attend(c, call, splits)
         assert np.isfinite(out).all()
         assert (np.abs(out - o).max(2) <= 1e-3 * np.abs(o).max(2)).all()
+
+
+# ---------------------------------------------------------------------------------------------------- a shared prefix
+def cascade(dev, S, H, gqa, shared, seed, exps, away=()):
+    """The cascade entry point over a raw prefix of `shared` groups whose V are 2^exps[g] (keys of the groups `away` along -8,
+    others along +8 on one channel if there are any), and own tokens like the last of them. Returns what came out, the
+    reference, its sums of p |v| and the bound on a weight's relative error."""
+    import torch
+    from chromofold_amd import kv
+    D, n = 128, 64 * shared
+    rng = np.random.default_rng(seed)
+    T = n + 5
+    exp = np.repeat(np.array(list(exps) + [exps[-1]], np.float32), 64)[:T]
+    k0 = rng.standard_normal((H, n, D)).astype(np.float32)
+    v0 = rng.standard_normal((H, n, D)).astype(np.float32) * np.exp2(exp[:n])[:, None]
+    data = []
+    for _ in range(S):
+        k1, v1 = (rng.standard_normal((H, 5, D)).astype(np.float32) for _ in range(2))
+        data.append((np.concatenate([k0, k1], 1), np.concatenate([v0, v1 * np.exp2(exp[n:])[:, None]], 1)))
+    q = rng.standard_normal((S, H * gqa, D)).astype(np.float32)
+    scale = D ** -0.5
+    if len(away):
+        scale, q[:, :, 0] = 10.0, 1.0
+        side = np.repeat(np.array([-8.0 if g in away else 8.0 for g in range(shared + 1)], np.float32), 64)[:T]
+        for k, _ in data:
+            k *= np.float32(0.02)
+            k[..., 0] = side
+    tables = np.concatenate([kv.build_table(x[h][:128].reshape(-1, 16, D)) for h in range(H) for x in (k0, v0 + 1)])
+    kvb = kv.build_batched(kv.CODEC_RANS_HYBRID, lambda s: data[s], S, H, np.full(S, T), D, tables, dev,
+                           shared={s: (0, shared) for s in range(1, S)}, raw_groups={0: shared})
+    out = torch.full(q.shape, float("nan"), device=dev)
+    kvb.attention(up(dev, q), out, up(dev, np.full(S, T - 1, np.uint32)), scale, splits=1, shared_groups=shared)
+
+    def dequant(x):
+        x = torch.from_numpy(np.pad(x, ((0, 0), (0, -T % 16), (0, 0)))).view(H, -1, 16, D)
+        m = x.abs().amax(dim=(2, 3), keepdim=True)
+        s = torch.where(m == 0, torch.ones_like(m), m / 127.0)
+        return (torch.round(x / s).double() * s.double()).view(H, -1, D)[:, :T]
+    want, mag, big = np.zeros(q.shape), np.zeros(q.shape), 0.0
+    for s in range(S):
+        k, v = (dequant(x) for x in data[s])
+        x = torch.from_numpy(q[s]).double().view(H, gqa, D)
+        p = torch.softmax(torch.matmul(x, k.transpose(1, 2)) * scale, -1)
+        want[s], mag[s] = (torch.matmul(p, y).view(H * gqa, D).numpy() for y in (v, v.abs()))
+        big = max(big, float(torch.matmul(x.abs(), k.abs().transpose(1, 2)).max()) * scale)
+    # a weight's relative error is its score's absolute one: operands of 22 bits and float32 sums, 2^-21 of sum |q k|, and
+    # about 2^-20 for exp, the weights' own parts and the merge; twice that for numerator and sum
+    return down(out).astype(np.float64), want, mag, 2 * (2.0 ** -21 * big + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("gqa", [1, 4])
+def test_cascade_v_scales_that_fall_in_steps(dev, gqa):
+    # the prefix splits of 240 sequences behind 25 groups of 8 heads hold 5 groups (cu_count / 120 of them)
+    out, want, mag, e = cascade(dev, 240, 8, gqa, 25, 301, [30, -25, -80, -110, -110] * 5)
+    assert np.isfinite(out).all()
+    assert (np.abs(out - want) <= e * mag + 2.0 ** -39 * 2.0 ** 33 / 127 * 25 * 64).all()
+
+
+@pytest.mark.parametrize("gqa", [1, 4])
+def test_cascade_small_v_behind_large_v_of_no_weight(dev, gqa):
+    out, want, mag, e = cascade(dev, 240, 8, gqa, 25, 302, [20, -30, -60, -95, -100] * 5, [g for g in range(25) if g % 5 < 3])
+    # the units of the groups that count: 2^-92 / 127 at most, so 2^(-98 - 14); each weight 2^-25 of it off, times a symbol
+    floor = 2.0 ** (-25 - 98 - 14) * 128 * 25 * 64
+    assert (np.abs(out - want) <= e * mag + floor).all()
+    assert (np.abs(want) > 2 * floor).mean() > 0.9
