@@ -1160,11 +1160,13 @@ __global__ __launch_bounds__(kPfxThreads) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
       for (int r = 0; r < 4; ++r) st[G][r] = a[r] * ksc;
     }
+    uint32_t hidden = 0;  // pages of which the lane's row sees nothing
     // unless every row sees every token of the group
     if (tc01 != 0x00100010u || tc23 != 0x00100010u || vmin < 64u * (g + 1)) {
 #pragma unroll
       for (int G = 0; G < 4; ++G) {
         const uint32_t tcg = (G < 2 ? tc01 : tc23) >> (16 * (G & 1)) & 0xFFFFu;
+        if (tcg == 0 || 64u * g + 16u * G >= vis) hidden |= 1u << G;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint32_t tok = 4 * kg + r;
@@ -1233,7 +1235,8 @@ __global__ __launch_bounds__(kPfxThreads) __attribute__((amdgpu_waves_per_eu(2))
       const float mref = m == -INFINITY ? 0.0f : m;  // no token visible yet: every p is exp(-inf) = 0
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const float v = ldexpf(vscale[2 * s2 + u], -e_run);
+        // (0 where the page is hidden: its scale may be anything, and 0 * inf would be in the row's sums)
+        const float v = hidden >> (2 * s2 + u) & 1u ? 0.0f : ldexpf(vscale[2 * s2 + u], -e_run);
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
           const float p0 = __expf(st[2 * s2 + u][r] - mref), p1 = __expf(st[2 * s2 + u][r + 1] - mref);

@@ -175,10 +175,11 @@ def test_small_v_beside_absent_pages(dev, monkeypatch, codec, call, gqa, D):
 
 
 # ---------------------------------------------------------------------------------------------------- a shared prefix
-def cascade(dev, S, H, gqa, shared, seed, exps, away=()):
+def cascade(dev, S, H, gqa, shared, seed, exps, away=(), pos=None, edit=None):
     """The cascade entry point over a raw prefix of `shared` groups whose V are 2^exps[g] (keys of the groups `away` along -8,
-    others along +8 on one channel if there are any), and own tokens like the last of them. Returns what came out, the
-    reference, its sums of p |v| and the bound on a weight's relative error."""
+    others along +8 on one channel if there are any), and own tokens like the last of them; query positions `pos` (the last
+    token), and what edit(kvb) makes of the sealed cache. Returns what came out, the reference, its sums of p |v| and the
+    bound on a weight's relative error."""
     import torch
     from chromofold_amd import kv
     D, n = 128, 64 * shared
@@ -201,9 +202,12 @@ def cascade(dev, S, H, gqa, shared, seed, exps, away=()):
             k[..., 0] = side
     tables = np.concatenate([kv.build_table(x[h][:128].reshape(-1, 16, D)) for h in range(H) for x in (k0, v0 + 1)])
     kvb = kv.build_batched(kv.CODEC_RANS_HYBRID, lambda s: data[s], S, H, np.full(S, T), D, tables, dev,
-                           shared={s: (0, shared) for s in range(1, S)}, raw_groups={0: shared})
+                           shared={s: (0, shared) for s in range(1, S)}, raw_groups={0: shared}, keep_host=True)
+    if edit:
+        edit(kvb)
+    pos = np.full(S, T - 1, np.uint32) if pos is None else np.array(pos, np.uint32)
     out = torch.full(q.shape, float("nan"), device=dev)
-    kvb.attention(up(dev, q), out, up(dev, np.full(S, T - 1, np.uint32)), scale, splits=1, shared_groups=shared)
+    kvb.attention(up(dev, q), out, up(dev, pos), scale, splits=1, shared_groups=shared)
 
     def dequant(x):
         x = torch.from_numpy(np.pad(x, ((0, 0), (0, -T % 16), (0, 0)))).view(H, -1, 16, D)
@@ -212,7 +216,7 @@ def cascade(dev, S, H, gqa, shared, seed, exps, away=()):
         return (torch.round(x / s).double() * s.double()).view(H, -1, D)[:, :T]
     want, mag, big = np.zeros(q.shape), np.zeros(q.shape), 0.0
     for s in range(S):
-        k, v = (dequant(x) for x in data[s])
+        k, v = (dequant(x)[:, : int(pos[s]) + 1] for x in data[s])
         x = torch.from_numpy(q[s]).double().view(H, gqa, D)
         p = torch.softmax(torch.matmul(x, k.transpose(1, 2)) * scale, -1)
         want[s], mag[s] = (torch.matmul(p, y).view(H * gqa, D).numpy() for y in (v, v.abs()))
@@ -237,3 +241,22 @@ def test_cascade_small_v_behind_large_v_of_no_weight(dev, gqa):
     floor = 2.0 ** (-25 - 98 - 14) * 128 * 25 * 64
     assert (np.abs(out - want) <= e * mag + floor).all()
     assert (np.abs(want) > 2 * floor).mean() > 0.9
+
+
+@pytest.mark.parametrize("gqa", [1, 4])
+def test_cascade_scales_behind_the_query(dev, gqa):
+    """Queries that end inside the shared prefix, all of them before the pages whose scales are infinite or NaN; then two
+    that see them, whose rows alone are NaN."""
+    def edit(kvb):
+        for h in range(2):
+            o = 16 * int(kvb.host_offsets[0, h, 6])
+            kvb.pool[o + 56: o + 64] = up(dev, np.array([np.nan, np.inf], np.float32).view(np.uint8))
+            kvb.pool[o + 40: o + 48] = up(dev, np.full(2, np.nan, np.float32).view(np.uint8))
+    pos = [64 * 6 + 31, 64 * 6 + 3, 64 * 6, 64 * 5 + 40, 64 * 2 + 7] * 4
+    out, want, mag, e = cascade(dev, 20, 2, gqa, 10, 303, [0] * 10, pos=pos, edit=edit)
+    assert np.isfinite(out).all()
+    assert (np.abs(out - want) <= e * mag + 2.0 ** -39 * 8 / 127 * 127 * 640).all()
+    pos[7], pos[12] = 64 * 6 + 32, 64 * 10 - 1
+    out, _, _, _ = cascade(dev, 20, 2, gqa, 10, 303, [0] * 10, pos=pos, edit=edit)
+    nan = np.isnan(out).all(2)
+    assert nan[[7, 12]].all() and np.isfinite(out[[i for i in range(20) if i not in (7, 12)]]).all()
