@@ -136,6 +136,46 @@ def test_small_v_behind_large_v_of_no_weight(dev, monkeypatch, codec, call, gqa,
         assert (np.abs(o) > 2 * floor).mean() > 0.9
 
 
+ZERO_CALLS = [c for c in CALLS if c[:2] == (1, "selected")]
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("codec, call, gqa", ZERO_CALLS)
+@pytest.mark.parametrize("exp", [-20, -30, -44, 10])
+def test_pages_of_zeros_beside_small_v(dev, monkeypatch, codec, call, gqa, D, exp):
+    """Pages whose V are all 0, or whose tokens before the query are, among pages of V around 2^exp: whatever scale they have
+    (the encoders write 1; 2^25 and 0 too), the others keep their bits."""
+    lens, pos = [640, 390, 64, 700], [639, 389, 63, 64 * 10 + 16 * 2 + 4]
+
+    def edit(data):
+        rng = np.random.default_rng(7)
+        for s, (_, v) in enumerate(data):
+            v *= np.float32(2.0 ** exp)
+            for h in range(2):
+                for page in range(-(-lens[s] // 16)):
+                    if rng.random() < 0.4 and s != 2 or s == 2 and page in (0, 3):
+                        v[h, 16 * page: 16 * page + 16] = 0.0
+        data[3][1][:, 640: 640 + 37] = 0.0   # of the query's page only what lies behind it, and far larger
+        data[3][1][:, 640 + 16: 640 + 32] = np.float32(2.0 ** exp)
+        data[3][1][:, 640 + 37:] = 1.0
+    c = cache(monkeypatch, dev, lens, 2, gqa, D, 205, codec, edit, pos=pos)
+    for h in (0, 1):
+        zero = [p for p in range(40) if not c.v[0][h][16 * p: 16 * p + 16].any()]
+        for p, scale in zip(zero, [2.0 ** 25, 0.0] * 20):
+            o = 16 * int(c.kvb.host_offsets[0, h, p // 4]) + 48 + 4 * (p % 4)
+            c.kvb.pool[o: o + 4] = up(dev, np.array([scale], np.float32).view(np.uint8))
+    o, _, mag, big, _ = R.attend_ref(c.q, c.k, c.v, c.lens, c.pos, gqa, c.scale, None, 1, c.M)
+    # as kvselect_helpers.weight_floor, from the pages that hold something: scales of 2^exp / 127 to 6 times that
+    low = np.zeros(o.shape)
+    for s in range(4):
+        for h in (0, 1):
+            low[s, h * gqa: (h + 1) * gqa] = 2.0 ** -39 * 6 * np.abs(c.v[s][h][: pos[s] + 1]).sum(0)
+    tol = R.tolerance(big, D)[..., None] * mag + 2.0 ** -23 * np.abs(o) + low
+    for splits in (0, 1, 3):
+        out = attend(c, call, splits)
+        assert (np.abs(out - o) <= tol).all(), splits
+
+
 # ---------------------------------------------------------------------------------------------------- what is not visible
 @pytest.mark.parametrize("D", [128, 64])
 @pytest.mark.parametrize("codec, call, gqa", CALLS)
