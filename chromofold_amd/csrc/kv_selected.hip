@@ -978,12 +978,12 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
         };
         float p[kGqa];
         if (gcodec == CF_KV_CODEC_RANS_HYBRID)
-          group_body<D, CF_KV_CODEC_RANS_HYBRID, 0>(stage_next, pre, nlw, st, raw_of(here_blob, chain),
-                                                    reinterpret_cast<const uint16_t *>(buf), cnt, s_tab, qhi, qlo, qsum, s_p[wave],
-                                                    static_cast<uint32_t *>(nullptr), lane, tok_ok, ks, vs, unit, gqa, m_run, l_run,
-                                                    acc_v, static_cast<uint32_t *>(nullptr), false, p);
+          group_body<D, CF_KV_CODEC_RANS_HYBRID, 0, const uint16_t *, decltype(stage_next), false, false, false, true>(
+              stage_next, pre, nlw, st, raw_of(here_blob, chain), reinterpret_cast<const uint16_t *>(buf), cnt, s_tab, qhi, qlo,
+              qsum, s_p[wave], static_cast<uint32_t *>(nullptr), lane, tok_ok, ks, vs, unit, gqa, m_run, l_run, acc_v,
+              static_cast<uint32_t *>(nullptr), false, p);
         else
-          group_body<D, CF_KV_CODEC_INT8, 0, const uint16_t *>(
+          group_body<D, CF_KV_CODEC_INT8, 0, const uint16_t *, decltype(stage_next), false, false, false, true>(
               stage_next, pre, nlw, st, reinterpret_cast<const uint32_t *>(here_blob + cfkv::kHdr),
               static_cast<const uint16_t *>(nullptr), 0, s_tab, qhi, qlo, qsum, s_p[wave], static_cast<uint32_t *>(nullptr), lane,
               tok_ok, ks, vs, unit, gqa, m_run, l_run, acc_v, static_cast<uint32_t *>(nullptr), false, p);

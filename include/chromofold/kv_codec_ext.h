@@ -122,6 +122,8 @@ typedef struct cf_kv_group_header {
  * Results repeat bit for bit for the same descriptor contents and lengths. With splits = 0 the launch balances the batch
  * over the chip by the sequences' lengths, so that a row's fp32 rounding depends on the lengths of the others in the
  * batch (differences of about 1e-6 of a row); with splits given it depends on its own sequence alone.
+ * Within a group V is added up in units of the largest V scale of the pages with a visible token; a page of zeros, whose
+ * scale is 1, counts. Pages with a scale down to 2^-18 of that keep 22 bits, smaller ones fewer, below 2^-39 none.
  * The entry point allocates nothing and never synchronises. */
 typedef struct cf_kv_batched_desc {
     uint32_t struct_size;
