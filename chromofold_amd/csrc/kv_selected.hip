@@ -108,7 +108,8 @@ __device__ __forceinline__ uint32_t row_slots(const SelArgs &a, uint32_t ngroups
   return a.s.units ? min(a.slots, (ngroups + a.s.unit_groups - 1) / a.s.unit_groups * a.s.unit_groups) : ngroups;
 }
 
-// Weight of a group from its heads' statistics, the row's maxima and the inverse sums.
+// Weight of an attended group from its heads' statistics, the row's maxima and the inverse sums (0 of a group whose scores are
+// all -inf; a row of such groups has a NaN for its maximum).
 template <typename Stat>
 __device__ __forceinline__ float group_weight(const Stat &stat, uint32_t gqa, const float *m, const float *inv_l) {
   float w = 0.0f;
@@ -118,7 +119,7 @@ __device__ __forceinline__ float group_weight(const Stat &stat, uint32_t gqa, co
     for (uint32_t j = 0; j < 4; ++j) x[j] = stat(min(h0 + j, gqa - 1));
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j)
-      if (h0 + j < gqa && x[j].x != -INFINITY) w += x[j].y * __builtin_amdgcn_exp2f(x[j].x - m[h0 + j]) * inv_l[h0 + j];
+      if (h0 + j < gqa) w += x[j].y * __builtin_amdgcn_exp2f(x[j].x - m[h0 + j]) * inv_l[h0 + j];
   }
   return w;
 }
@@ -495,13 +496,16 @@ struct RowState {
   }
 
   // l becomes the sum over all lanes; m a NaN where the row is broken or holds one (a NaN score leaves the maximum as it was
-  // and makes the sum a NaN).
-  __device__ __forceinline__ void close() {
+  // and makes the sum a NaN). attended: whether a group was. Where every score was -inf, l is then 1 beside the maximum of -inf:
+  // unlike a state without a token, it makes a row NaN that has nothing else.
+  __device__ __forceinline__ void close(bool attended) {
     const bool broken = __builtin_amdgcn_ballot_w64(bad) != 0;
     Spread<GT>::reduce_sum(l);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r) {
+      if (attended && m[r] == -INFINITY && l[r] == 0.0f) l[r] = 1.0f;
       if (broken || l[r] != l[r]) m[r] = __builtin_nanf("");
+    }
   }
 
   // The closed state to memory, its sums in absolute units.
@@ -608,7 +612,7 @@ __global__ __launch_bounds__(64 * W, 2) void row_kernel(SelArgs a) {
     if (!ROW && stats) write_stats(a.stats + row * a.slots * gqa, lds.stat, mine, min(step, w1 - c0), gqa);
   }
   st.bad |= bad;
-  st.close();
+  st.close(!ROW && split_done);
   // ---- join the wavefronts
   if (n == 0) {
 #pragma unroll
@@ -643,6 +647,12 @@ __global__ __launch_bounds__(64 * W, 2) void row_kernel(SelArgs a) {
         l += s_l[w][h] * f;
         o += sh.red[w][h][dd] * f;
       }
+    if constexpr (ROW) {  // lists ascend: the first entry is visible if any is
+      if (m == -INFINITY && nslots) nan |= listed_group(a, list, 0, bad) < ngroups;
+    } else if (m == -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) l += s_l[w][h];  // (not 0 where all scores are -inf: see close())
+    }
     if (nan) m = __builtin_nanf("");
     if constexpr (ROW) {
       a.d.output[(static_cast<size_t>(seq) * a.d.query_head_count + head * gqa + h) * D + dd] =
@@ -766,7 +776,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
     if (!first)
       for (; row != r; ++row) {
         st.bad |= row_broken();
-        st.close();
+        st.close(q_row == row);
         const size_t state = static_cast<size_t>(me) + row;
         st.store(a.sums + state * gqa * D, a.states + state * gqa, gqa);
         st.reset();
@@ -1107,10 +1117,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a, uint32_t 
   // a wavefront per query head: its maximum and the inverse of its sum
   for (uint32_t h = every ? tid >> 6 : blockIdx.z; h < (every ? gqa : blockIdx.z + 1); h += kJoinThreads / 64) {
     float m = -INFINITY, l = 0.0f;
-    bool nan = false;
+    bool nan = false, low = false;  // low: a state whose scores were all -inf
     for (uint32_t s = lane; s < states; s += 64) {
       const float2 x = st[static_cast<size_t>(s) * gqa + h];
       nan |= x.x != x.x;
+      low |= x.x == -INFINITY && x.y != 0.0f;
       const float mn = fmaxf(m, x.x);
       if (mn != -INFINITY) {
         l = (m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - mn)) +
@@ -1121,7 +1132,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(SelArgs a, uint32_t 
     const float top = cfd::rows4_max(cfd::row16_max(m));
     l = m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - top);
     l = cfd::rows4_sum(cfd::row16_sum(l));
-    nan = __builtin_amdgcn_ballot_w64(nan) != 0;
+    nan = __builtin_amdgcn_ballot_w64(nan || (top == -INFINITY && low)) != 0;
     if (lane == 0) {
       s_m[h] = nan ? __builtin_nanf("") : top;
       s_inv[h] = 1.0f / l;

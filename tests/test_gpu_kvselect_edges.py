@@ -214,6 +214,70 @@ def test_small_v_beside_absent_pages(dev, monkeypatch, codec, call, gqa, D):
         assert (np.abs(out - o).max(2) <= 1e-3 * np.abs(o).max(2)).all()
 
 
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("gqa", [1, 4, 7, 16])
+def test_scores_of_minus_infinity(dev, monkeypatch, gqa, D):
+    """K scales of +inf with products below 0 in all pages (row 0), in some of them (1), in none (2), and in all but with one
+    query head whose products are above 0 (3); row 4 has no tokens. Heads whose scores are all -inf are NaN, and so are the
+    weights of their groups; others are as if those tokens were not there."""
+    def edit(data):
+        for k, _ in data:
+            k[:] = 0.0
+            k[..., 0] = 1.0
+    lens = [300, 300, 300, 300, 0]
+    c = cache(monkeypatch, dev, lens, 2, gqa, D, 206, 1, edit)
+    gone = {0: range(19), 1: [0, 1, 2, 3, 9, 14], 2: [], 3: range(19)}
+    inf = up(dev, np.array([np.inf], np.float32).view(np.uint8))
+    for s, pages in gone.items():
+        for h in (0, 1):
+            for p in pages:
+                o = 16 * int(c.kvb.host_offsets[s, h, p // 4]) + 32 + 4 * (p % 4)
+                c.kvb.pool[o: o + 4] = inf
+    c.q[:] = 0.0
+    c.q[:, :, 0] = -1.0
+    if gqa > 1:
+        c.q[3, 1, 0] = 0.5  # inf - inf
+    left = [[x.copy() for x in c.k[1]], [x.copy() for x in c.v[1]]]
+    keep = ~np.isin(np.arange(300) // 16, gone[1])
+    for units, unit in ((None, 1), (np.tile(np.arange(5, dtype=np.uint32), (5, 2, 1)), 1)):
+        for splits in (0, 1, 3):
+            out, w = c.run(units, unit, weights=None, splits=splits)
+            assert np.isnan(out[[0, 3]]).all() and np.isnan(w[[0, 3]]).all(), splits
+            assert np.isfinite(out[[1, 2, 4]]).all() and np.isfinite(w[[1, 2, 4]]).all(), splits
+            assert (out[4] == 0).all() and (w[4] == 0).all()
+            for h in (0, 1):  # equal scores: means over the tokens that are left, 1 / n of the weight each
+                v, g = left[1][h][keep], np.bincount(np.arange(300)[keep] // 64, minlength=c.M)
+                bound = (R.tolerance(1.0 / np.sqrt(D), D) + 2.0 ** -23) * np.abs(v).mean(0) + R.weight_floor(left[1][h], np.arange(300))
+                assert (np.abs(out[1, h * gqa: (h + 1) * gqa] - v.mean(0)) <= bound).all()
+                assert (np.abs(w[1, h] - gqa * g / keep.sum()) <= R.tolerance(1.0 / np.sqrt(D), D) * gqa * g / keep.sum()).all()
+
+
+def test_many_rows_of_minus_infinity(dev, monkeypatch):
+    # the cut into stretches over several rows: every third row's K scales are +inf, every seventh row is empty
+    def edit(data):
+        for k, _ in data:
+            k[:] = 1.0
+    rng = np.random.default_rng(8)
+    S, M = 600, 60
+    lens = [0 if s % 7 == 3 else int(x) for s, x in enumerate(rng.integers(1, 300, S))]
+    lens[300] = 64 * M
+    c = cache(monkeypatch, dev, lens, 1, 4, 64, 207, 1, edit)
+    inf = up(dev, np.full(4, np.inf, np.float32).view(np.uint8))
+    for s in range(0, S, 3):
+        for g in range(-(-lens[s] // 64)):
+            o = 16 * int(c.kvb.host_offsets[s, 0, g])
+            c.kvb.pool[o + 32: o + 48] = inf
+    c.q[:] = -1.0
+    out, w = c.run()
+    none = np.array(lens) == 0
+    low = (np.arange(S) % 3 == 0) & ~none
+    assert np.isnan(out[low]).all() and (out[none] == 0).all() and np.isfinite(out[~low]).all()
+    for s in np.flatnonzero(low):
+        n = -(-lens[s] // 64)
+        assert np.isnan(w[s, 0, :n]).all() and (w[s, 0, n:] == 0).all()
+    assert np.isfinite(w[~low]).all()
+
+
 # ---------------------------------------------------------------------------------------------------- a shared prefix
 def cascade(dev, S, H, gqa, shared, seed, exps, away=(), pos=None, edit=None):
     """The cascade entry point over a raw prefix of `shared` groups whose V are 2^exps[g] (keys of the groups `away` along -8,
