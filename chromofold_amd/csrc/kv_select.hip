@@ -91,7 +91,9 @@ __global__ __launch_bounds__(64 * kBoundWaves) void key_bounds_kernel(
     float top = fmaxf(fmaxf(fmaxf(hi[0], lo[0]), fmaxf(hi[1], lo[1])), fmaxf(fmaxf(hi[2], lo[2]), fmaxf(hi[3], lo[3])));
 #pragma unroll
     for (int o = 1; o < kL; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float s = bad ? INFINITY : top / 127.0f;
+    float s = bad ? INFINITY : top / 127.0f;
+    // a subnormal quotient may have lost up to a third to rounding (all, from 0.5 steps down): up, so that 127 s is not below top
+    if (s < 0x1p-126f && __builtin_fmaf(s, 127.0f, -top) < 0.0f) s = __uint_as_float(__float_as_uint(s) + 1);
     uint32_t ch = 0, cl = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

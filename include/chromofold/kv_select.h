@@ -36,7 +36,8 @@ extern "C" {
 #define CF_KV_SELECT_MAX_GQA 16u       /* query heads per KV head (attention over RANS_HYBRID pools: 4) */
 
 /* ---- key bounds ------------------------------------------------------------------------------------------------
- * Record of a group, head_dim D: scale s = max |k| / 127 over its tokens and channels; 2 D codes,
+ * Record of a group, head_dim D: scale s = max |k| / 127 over its tokens and channels (rounded up where s is subnormal: to
+ * nearest, 127 s could be far below the maximum); 2 D codes,
  *   codes[d]     = min(127, ceil( max_t k[t][d] / s))      an upper bound on channel d in steps of s
  *   codes[D + d] = min(127, ceil(-min_t k[t][d] / s))      a lower bound, negated
  * (IEEE fp32 quotients; codes are in [-127, 127]). A group of zeros has scale 0 and codes 0; one that holds an infinity or

@@ -51,6 +51,33 @@ def test_seal_device_on_another_stream(dev):
         assert torch.equal(out, ref)
 
 
+# ---------------------------------------------------------------------------------------------------- key bounds
+@pytest.mark.parametrize("D", [128, 64])
+def test_bounds_bound_every_finite_group(dev, D):
+    """Groups from the least subnormal key to the largest finite one, whole and cut: scale times code is never inside the keys
+    by more than the quotient's and the scale's rounding, 2^-23 of the scale's 127 steps, and a scale of 0 means zeros."""
+    from chromofold_amd import kvselect as ks
+    rng = np.random.default_rng(D)
+    least = np.float64(2.0 ** -149)
+    tops = [least * n for n in (1, 2, 63, 64, 100, 126, 127, 128, 180, 190, 191, 254, 300, 1000, 12345, 127 * 2 ** 23 - 1)]
+    tops += [127 * 2.0 ** -126, 2.0 ** -126, 1e-20, 1.0, 3.3e38]
+    groups = []
+    for top in tops:
+        k = (rng.uniform(-1, 1, (64, D)) * top).astype(np.float32)
+        k[rng.integers(64), rng.integers(D)] = np.float32(top)
+        k[rng.integers(64), rng.integers(D)] = -np.float32(top)
+        groups.append(k)
+    keys, n = np.concatenate(groups).reshape(-1, 16, D), len(groups)
+    out = ks.empty_bounds(1, 1, n, D, dev)
+    ks.key_bounds(up(dev, keys), up(dev, 4 * np.arange(n, dtype=np.int64)), up(dev, np.full(n, 4, np.uint32)), out)
+    codes, scales = down(out.codes)[0, 0].astype(np.float64), down(out.scales)[0, 0].astype(np.float64)
+    for k, c, s in zip(groups, codes, scales):
+        k, slack = k.astype(np.float64), 2.0 ** -23 * 127 * s
+        assert (c[:D] * s >= k.max(0) - slack).all() and (c[D:] * s >= -k.min(0) - slack).all(), (np.abs(k).max(), s)
+        assert (c[:D] * s <= k.max(0) + s + slack).all() and (c[D:] * s <= -k.min(0) + s + slack).all()
+        assert s > 0
+
+
 # ---------------------------------------------------------------------------------------------------- V scales
 def cache(monkeypatch, dev, lens, H, gqa, D, seed, codec=1, edit=None, **how):
     """A Case whose data `edit(data)` may change before it is sealed (coded pools as chain pairs)."""
