@@ -6,7 +6,8 @@
   evict        the groups of least accumulated weight leave the page tables         cf_kv_evict_groups_async
 
 u32 arrays are int32 tensors of the same bits; -1 is CF_KV_NO_UNIT. The *_desc functions make a descriptor to be kept for
-repeated calls (and as long as a graph captured with it); it holds the tensors it points at."""
+repeated calls (and as long as a graph captured with it); it holds the tensors it points at. What a call is given beside one
+has to be what the descriptor was made of: other tensors or numbers are refused (None and defaults are not looked at)."""
 from __future__ import annotations
 
 import contextlib
@@ -118,6 +119,17 @@ def _with_workspace(desc, need: int, device: torch.device, stream) -> None:
             kv._give_workspace(desc, need, device, stream if stream is not None else torch.cuda.current_stream(device))
 
 
+def _kept(d, tensors: tuple, numbers: tuple, defaults: tuple) -> None:
+    """Refuses a call whose arguments are not those of the descriptor it brings: the call would read and write the
+    descriptor's. tensors in the order of d.held, from the first on; numbers in that of d.numbers."""
+    for t, h in zip(tensors, d.held):
+        if t is not h and t is not None and (h is None or t.data_ptr() != h.data_ptr() or t.shape != h.shape):
+            raise ValueError(f"a tensor of shape {tuple(t.shape)} is not the descriptor's: make a descriptor for it")
+    for x, n, default in zip(numbers, d.numbers, defaults):
+        if x != n and x != default and not (isinstance(n, float) and C.c_float(x).value == C.c_float(n).value):
+            raise ValueError(f"{x} is not the descriptor's {n}: make a descriptor for it")
+
+
 def _for_stream(d, cls, device: torch.device, stream, s: int):
     """The descriptor, or a copy with a workspace of its own where it was made for another stream than s."""
     if d.workspace and d.workspace_stream != s:
@@ -206,7 +218,8 @@ def select_desc(kvb: kv.BatchedKv, bounds: KeyBounds, queries: torch.Tensor, que
     d = cf_kv_select_desc(C.sizeof(cf_kv_select_desc), SELECT_ABI_VERSION, S, H, queries.shape[1], kvb.head_dim, M, unit_groups,
                           units.shape[2], keep_first, keep_last, 0, bounds.codes.data_ptr(), bounds.scales.data_ptr(),
                           kvb.seq_tokens.data_ptr(), query_pos.data_ptr(), queries.data_ptr(), units.data_ptr())
-    d.held = (bounds, kvb.seq_tokens, query_pos, queries, units)
+    d.held = (bounds.codes, bounds.scales, kvb.seq_tokens, query_pos, queries, units)
+    d.numbers = (unit_groups, keep_first, keep_last)
     A.check(A.lib().cf_kv_validate_select_desc(C.byref(d)), "cf_kv_validate_select_desc")
     _with_workspace(d, int(_on_device(dev, A.lib().cf_kv_select_workspace_bytes, C.byref(d))), dev, stream)
     return d
@@ -217,8 +230,12 @@ def select(kvb: kv.BatchedKv, bounds: KeyBounds, queries: torch.Tensor, query_po
            desc: cf_kv_select_desc | None = None) -> torch.Tensor:
     """Fills units int32 [seq_count, kv_heads, max_units] with the units of each row whose bound on the scores of `queries`
     [seq_count, query_heads, D] is largest, the first keep_first and the last keep_last always, ascending, then NO_UNIT."""
-    d = desc if desc is not None else select_desc(kvb, bounds, queries, query_pos, units, unit_groups, keep_first,
-                                                  keep_last, stream)
+    if desc is not None:
+        d = desc
+        _kept(d, (bounds.codes, bounds.scales, kvb.seq_tokens, query_pos, queries, units), (unit_groups, keep_first, keep_last),
+              (1, 1, 1))
+    else:
+        d = select_desc(kvb, bounds, queries, query_pos, units, unit_groups, keep_first, keep_last, stream)
     dev = kvb.group_offsets.device
     s = _raw_stream(dev, stream)
     _call("cf_kv_select_groups_async", dev, s, C.byref(_for_stream(d, cf_kv_select_desc, dev, stream, s)))
@@ -251,7 +268,8 @@ def attention_desc(kvb: kv.BatchedKv, queries: torch.Tensor, output: torch.Tenso
                               splits)
     d.selection = cf_kv_selection(C.sizeof(cf_kv_selection), SELECT_ABI_VERSION, unit_groups,
                                   0 if units is None else units.shape[2], _ptr(units), _ptr(weights), _ptr(weights_out), decay)
-    d.held = (kvb, queries, output, query_pos, units, weights, weights_out, d.selection)
+    d.held = (kvb.pool, kvb.group_offsets, kvb.seq_tokens, kvb.tables, queries, output, query_pos, units, weights, weights_out)
+    d.numbers = (float(softmax_scale), unit_groups, float(decay), splits)
     A.check(A.lib().cf_kv_validate_selection(C.byref(d), C.byref(d.selection)), "cf_kv_validate_selection")
     need = _on_device(dev, A.lib().cf_kv_selected_workspace_bytes, C.byref(d), C.byref(d.selection))
     _with_workspace(d, int(need), dev, stream)
@@ -266,8 +284,13 @@ def attention(kvb: kv.BatchedKv, queries: torch.Tensor, output: torch.Tensor, qu
     (optional; may be `weights`) becomes decay * weights (None: 0) + each group's share of the softmax weight, summed over
     the KV head's query heads."""
     dev = kvb.group_offsets.device
-    d = desc if desc is not None else attention_desc(kvb, queries, output, query_pos, softmax_scale, units, unit_groups, weights,
-                                                     weights_out, decay, splits, stream)
+    if desc is not None:
+        d = desc
+        _kept(d, (kvb.pool, kvb.group_offsets, kvb.seq_tokens, kvb.tables, queries, output, query_pos, units, weights,
+                  weights_out), (softmax_scale, unit_groups, decay, splits), (None, 1, 1.0, 0))
+    else:
+        d = attention_desc(kvb, queries, output, query_pos, softmax_scale, units, unit_groups, weights, weights_out, decay,
+                           splits, stream)
     s = _raw_stream(dev, stream)
     _call("cf_kv_paged_attention_selected_async", dev, s, C.byref(_for_stream(d, kv.cf_kv_batched_desc, dev, stream, s)),
           C.byref(d.selection))
@@ -283,6 +306,17 @@ class Evicted:
     weights: torch.Tensor | None = None
     bounds: KeyBounds | None = None
     dropped: torch.Tensor | None = None
+
+
+def _evicted(kvb: kv.BatchedKv, weights: torch.Tensor, out: Evicted | None, bounds: KeyBounds | None) -> tuple:
+    """The tensors of an eviction, None for those that are not there."""
+    o, b = out if out is not None else _NO_OUT, bounds if bounds is not None else _NO_BOUNDS
+    r = o.bounds if o.bounds is not None else _NO_BOUNDS
+    return (kvb.group_offsets, kvb.seq_tokens, weights, o.group_offsets, o.seq_tokens, o.weights, o.dropped, b.codes, b.scales,
+            r.codes, r.scales)
+
+
+_NO_BOUNDS, _NO_OUT = KeyBounds(None, None), Evicted(None, None)
 
 
 def evict_desc(kvb: kv.BatchedKv, weights: torch.Tensor, budget_units: int, out: Evicted | None = None,
@@ -310,7 +344,8 @@ def evict_desc(kvb: kv.BatchedKv, weights: torch.Tensor, budget_units: int, out:
                          keep_first, keep_last, kvb.group_offsets.data_ptr(), kvb.seq_tokens.data_ptr(), weights.data_ptr(),
                          rec[0], rec[1], out.group_offsets.data_ptr(), out.seq_tokens.data_ptr(), _ptr(out.weights), rec[2],
                          rec[3], _ptr(out.dropped))
-    d.held = (kvb.group_offsets, kvb.seq_tokens, weights, bounds, out)
+    d.held = _evicted(kvb, weights, out, bounds)
+    d.numbers = (budget_units, unit_groups, keep_first, keep_last)
     A.check(A.lib().cf_kv_validate_evict_desc(C.byref(d)), "cf_kv_validate_evict_desc")
     return d
 
@@ -321,6 +356,10 @@ def evict(kvb: kv.BatchedKv, weights: torch.Tensor, budget_units: int, out: Evic
     """Cuts every sequence with more than budget_units units back to that many per KV head: the first keep_first, the last
     keep_last, then those of the largest accumulated `weights`. out=None evicts in place: kvb's tables and lengths, weights
     and bounds."""
-    d = desc if desc is not None else evict_desc(kvb, weights, budget_units, out, bounds, unit_groups, keep_first, keep_last)
+    if desc is not None:
+        d = desc
+        _kept(d, _evicted(kvb, weights, out, bounds), (budget_units, unit_groups, keep_first, keep_last), (None, 1, 1, 1))
+    else:
+        d = evict_desc(kvb, weights, budget_units, out, bounds, unit_groups, keep_first, keep_last)
     dev = kvb.group_offsets.device
     _call("cf_kv_evict_groups_async", dev, _raw_stream(dev, stream), C.byref(d))

@@ -116,3 +116,114 @@ def test_seal_device_orders_its_two_streams(monkeypatch):
     st.log.clear()
     kv.seal_device(kv.CODEC_INT8, x, x, None)
     assert not any(y[0] == "wait" for y in st.log)
+
+
+# ---------------------------------------------------------------------------------------------------- kept descriptors
+S, H, M, D, K = 2, 3, 5, 64, 4
+
+
+def z(*shape, t=torch.int32):
+    return torch.zeros(*shape, dtype=t)
+
+
+class Kept:
+    """A cache of S sequences, its bounds and a step's tensors, and the three operators' calls with descriptors of them."""
+
+    def __init__(self):
+        self.kvb = kv.BatchedKv(kv.CODEC_INT8, S, H, D, M, z(64, t=torch.uint8), z(S, H, M), z(S), None)
+        self.b, self.to_b = ks.empty_bounds(S, H, M, D, "cpu"), ks.empty_bounds(S, H, M, D, "cpu")
+        f = torch.float32
+        self.q, self.out, self.pos, self.units = z(S, 2 * H, D, t=f), z(S, 2 * H, D, t=f), z(S), z(S, H, K)
+        self.w, self.w2 = z(S, H, M, t=f), z(S, H, M, t=f)
+        self.to = ks.Evicted(z(S, H, M), z(S), z(S, H, M, t=f), self.to_b, z(S, H, M))
+
+    def select(self, desc=None, **kw):
+        a = {"kvb": self.kvb, "bounds": self.b, "queries": self.q, "query_pos": self.pos, "units": self.units}
+        number = {"unit_groups": 2, "keep_first": 2, "keep_last": 1} if desc is None else {}
+        return (ks.select_desc if desc is None else ks.select)(**{**a, **number, **kw}, **({"desc": desc} if desc else {}))
+
+    def attention(self, desc=None, **kw):
+        a = {"kvb": self.kvb, "queries": self.q, "output": self.out, "query_pos": self.pos, "softmax_scale": 0.1}
+        more = {"units": self.units, "unit_groups": 2, "weights": self.w, "weights_out": self.w2, "decay": 0.9, "splits": 3}
+        return (ks.attention_desc if desc is None else ks.attention)(**{**a, **(more if desc is None else {}), **kw},
+                                                                     **({"desc": desc} if desc else {}))
+
+    def evict(self, desc=None, **kw):
+        a = {"kvb": self.kvb, "weights": self.w, "budget_units": 2}
+        more = {"out": self.to, "bounds": self.b, "unit_groups": 2, "keep_first": 0, "keep_last": 2}
+        return (ks.evict_desc if desc is None else ks.evict)(**{**a, **(more if desc is None else {}), **kw},
+                                                             **({"desc": desc} if desc else {}))
+
+
+@pytest.fixture
+def made(monkeypatch):
+    """Calls get as far as the library, which notes them."""
+    calls = []
+    monkeypatch.setattr(ks, "_raw_stream", lambda device, stream: 0)
+    monkeypatch.setattr(ks, "_for_stream", lambda d, *rest: d)
+    monkeypatch.setattr(ks, "_with_workspace", lambda *args: None)
+    monkeypatch.setattr(ks, "_call", lambda name, *rest: calls.append(name))
+    k = Kept()
+    k.calls = calls
+    return k
+
+
+def other(t):
+    return torch.zeros_like(t)
+
+
+def test_a_kept_descriptor_takes_its_own_arguments(made):
+    k = made
+    sd, ad, ed = k.select(), k.attention(), k.evict()
+    k.select(sd)
+    k.select(sd, units=k.units.view(S, H, K), unit_groups=2, keep_first=2)
+    k.attention(ad)
+    k.attention(ad, units=k.units, weights=k.w, weights_out=k.w2, decay=0.9, splits=3, unit_groups=2)
+    k.attention(ad, softmax_scale=float(torch.tensor(0.1)))  # the same as float32
+    k.evict(ed)
+    k.evict(ed, out=k.to, bounds=k.b, unit_groups=2, keep_first=0, keep_last=2)
+    assert k.calls == ["cf_kv_select_groups_async"] * 2 + ["cf_kv_paged_attention_selected_async"] * 3 + [
+        "cf_kv_evict_groups_async"] * 2
+
+
+def test_a_kept_descriptor_refuses_other_arguments(made):
+    k = made
+    sd, ad, ed = k.select(), k.attention(), k.evict()
+    cache = lambda **kw: kv.BatchedKv(**{**{f: getattr(k.kvb, f) for f in ("codec", "seq_count", "kv_heads", "head_dim",  # noqa
+                                                                          "max_groups", "pool", "group_offsets", "seq_tokens",
+                                                                          "tables")}, **kw})
+    bad = [
+        lambda: k.select(sd, queries=other(k.q)), lambda: k.select(sd, query_pos=other(k.pos)),
+        lambda: k.select(sd, units=other(k.units)), lambda: k.select(sd, bounds=k.to_b), lambda: k.select(sd, unit_groups=3),
+        lambda: k.select(sd, kvb=cache(seq_tokens=z(S))), lambda: k.select(sd, keep_first=3), lambda: k.select(sd, keep_last=2),
+        lambda: k.select(sd, units=k.units[:, :, :2]),
+        lambda: k.attention(ad, queries=other(k.q)), lambda: k.attention(ad, output=other(k.out)),
+        lambda: k.attention(ad, query_pos=other(k.pos)), lambda: k.attention(ad, softmax_scale=0.2),
+        lambda: k.attention(ad, units=other(k.units)), lambda: k.attention(ad, weights=k.w2),
+        lambda: k.attention(ad, weights_out=k.w), lambda: k.attention(ad, decay=0.5), lambda: k.attention(ad, splits=1),
+        lambda: k.attention(ad, kvb=cache(pool=z(64, t=torch.uint8))),
+        lambda: k.attention(ad, kvb=cache(group_offsets=z(S, H, M))),
+        lambda: k.attention(ad, kvb=cache(tables=z(64, t=torch.uint8))),
+        lambda: k.evict(ed, weights=k.w2), lambda: k.evict(ed, budget_units=3), lambda: k.evict(ed, bounds=k.to_b),
+        lambda: k.evict(ed, out=ks.Evicted(z(S, H, M), k.to.seq_tokens)), lambda: k.evict(ed, kvb=cache(seq_tokens=z(S))),
+        lambda: k.evict(ed, keep_last=3),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError, match="the descriptor"):
+            call()
+    assert not k.calls
+
+
+def test_a_kept_descriptor_holds_what_it_points_at(made):
+    # tensors of a cache whose fields are given others live as long as the descriptor
+    import weakref
+    k = made
+    refs = [weakref.ref(t) for t in (k.kvb.pool, k.kvb.group_offsets, k.kvb.seq_tokens, k.b.codes, k.to.weights)]
+    descs = [k.select(), k.attention(), k.evict()]
+    k.kvb.pool, k.kvb.group_offsets, k.kvb.seq_tokens = z(64, t=torch.uint8), z(S, H, M), z(S)
+    k.b.codes, k.to.weights = None, None
+    assert all(r() is not None for r in refs)
+    with pytest.raises(ValueError, match="the descriptor"):
+        k.attention(descs[1])
+    descs.clear()
+    assert all(r() is None for r in refs)
