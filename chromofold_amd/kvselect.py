@@ -200,6 +200,15 @@ def _check_cache(kvb: kv.BatchedKv) -> tuple:
     return dev, shape
 
 
+def _check_blobs(kvb: kv.BatchedKv, dev) -> None:
+    """The pool, and the tables where it is coded: two of each KV head."""
+    _need(kvb.pool, "pool", torch.uint8, kvb.pool.shape, dev)
+    if kvb.codec == kv.CODEC_RANS_HYBRID and kvb.tables is not None:
+        _need(kvb.tables, "tables", torch.uint8, kvb.tables.shape, dev)
+        if kvb.tables.numel() < 2 * kvb.kv_heads * kv.TABLE_BYTES:
+            raise ValueError(f"tables: {2 * kvb.kv_heads} of {kv.TABLE_BYTES} bytes are needed, got {kvb.tables.numel()} bytes")
+
+
 def _check_bounds(b: KeyBounds, name: str, shape: tuple, D: int, dev) -> KeyBounds:
     _need(b.codes, name + ".codes", torch.int8, (*shape, 2 * D), dev)
     _need(b.scales, name + ".scales", torch.float32, shape, dev)
@@ -249,6 +258,7 @@ def attention_desc(kvb: kv.BatchedKv, queries: torch.Tensor, output: torch.Tenso
                    splits: int = 0, stream=None) -> kv.cf_kv_batched_desc:
     """Descriptor for attention() (the batched one, its `selection` beside it), with a workspace for calls on `stream`."""
     dev, shape = _check_cache(kvb)
+    _check_blobs(kvb, dev)
     S, H, M = shape
     q = (S, queries.shape[1], kvb.head_dim)
     _need(queries, "queries", torch.float32, q, dev)

@@ -172,6 +172,29 @@ def other(t):
     return torch.zeros_like(t)
 
 
+def test_attention_checks_the_pool_and_the_tables(made):
+    u8 = torch.uint8
+    k, enough = made, 2 * H * kv.TABLE_BYTES
+
+    def cache(codec=kv.CODEC_INT8, pool=z(64, t=u8), tables=None):
+        k.kvb = kv.BatchedKv(codec, S, H, D, M, pool, z(S, H, M), z(S), tables)
+        return k.attention()
+    cache()
+    cache(kv.CODEC_RANS_HYBRID, tables=z(enough, t=u8))
+    cache(kv.CODEC_RANS_HYBRID, tables=z(2 * H, kv.TABLE_BYTES, t=u8))
+    cache(tables=z(1))  # not read
+    cache(pool=z(4, 16, t=u8))
+    rans = lambda tables: cache(kv.CODEC_RANS_HYBRID, tables=tables)  # noqa: E731
+    for bad in (lambda: cache(pool=z(16)), lambda: cache(pool=z(128, t=u8)[::2]),
+                lambda: cache(pool=torch.empty(64, dtype=u8, device="meta")), lambda: rans(z(enough // 4)),
+                lambda: rans(z(enough - 1, t=u8)), lambda: rans(z(2 * enough, t=u8)[::2]),
+                lambda: rans(torch.empty(enough, dtype=u8, device="meta"))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(A.CfError):
+        rans(None)
+
+
 def test_a_kept_descriptor_takes_its_own_arguments(made):
     k = made
     sd, ad, ed = k.select(), k.attention(), k.evict()
