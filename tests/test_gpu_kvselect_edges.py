@@ -6,7 +6,7 @@ import pytest
 import kvselect_helpers as R
 import test_gpu_kvselect as T
 from kv_helpers import make_seqs
-from test_gpu_kvselect import dev, down, up  # noqa: F401 (dev: the fixture)
+from test_gpu_kvselect import dev, down, u32, up  # noqa: F401 (dev: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -49,6 +49,60 @@ def test_seal_device_on_another_stream(dev):
         assert torch.equal(got.group_offsets, want.group_offsets) and got.pool.numel() == want.pool.numel()
         got.attention(q, out, pos, 0.125)
         assert torch.equal(out, ref)
+
+
+def test_every_stream_has_a_workspace(dev, monkeypatch):
+    """Calls of one descriptor on several streams, which may overlap: on its own stream it brings its workspace, on every other
+    one a copy with one that is that call's. A selection of two launches and an attention of split rows; results as on one
+    stream."""
+    import torch
+    from chromofold_amd import kvselect as ks
+    rng = np.random.default_rng(9)
+    S, H, M, D = 2, 2, 1100, 128
+    codes, scales = T._records(rng, S, H, M, D)
+    c = T.Case(dev, [64 * 40, 64 * 33 + 1], H, 4, D, 62)
+    b = ks.KeyBounds(up(dev, codes), up(dev, scales))
+    long = T._cache(dev, S, H, D, M, [64 * M, 64 * M - 70])
+    q, pos, q2 = up(dev, c.q), up(dev, np.array(c.pos, np.uint32)), up(dev, rng.standard_normal((S, 2 * H, D)).astype(np.float32))
+    far = up(dev, np.array([64 * M - 1, 64 * M - 1], np.uint32))
+    units, out, w = torch.empty(S, H, 70, dtype=torch.int32, device=dev), torch.empty_like(q), torch.empty(S, H, c.M, device=dev)
+    own = torch.cuda.Stream(dev)
+    own.wait_stream(torch.cuda.current_stream(dev))
+    sd = ks.select_desc(long, b, q2, far, units, stream=own)
+    ad = ks.attention_desc(c.kvb, q, out, pos, c.scale, weights_out=w, splits=4, stream=own)
+    assert sd.workspace and ad.workspace
+    used, inner = [], ks._for_stream
+
+    def for_stream(d, cls, device, stream, s):
+        got = inner(d, cls, device, stream, s)
+        used.append((d, got, s))
+        return got
+    monkeypatch.setattr(ks, "_for_stream", for_stream)
+
+    def calls(stream):
+        ks.select(long, b, q2, far, units, desc=sd, stream=stream)
+        ks.attention(c.kvb, q, out, pos, c.scale, desc=ad, stream=stream)
+    calls(own)
+    own.synchronize()
+    want = [x.clone() for x in (units, out, w)]
+    assert np.array_equal(u32(units), R.select_ref(down(q2), codes, scales, [64 * M, 64 * M - 70], [64 * M - 1] * 2, 2, 1, 70, 1, 1))
+    c.compare(R.attend_ref(c.q, c.k, c.v, c.lens, c.pos, 4, c.scale, None, 1, c.M), down(out).astype(np.float64),
+              down(w).astype(np.float64))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(3)]
+    for st in streams + [None, own]:
+        calls(st)
+    torch.cuda.synchronize()
+    for a, e in zip((units, out, w), want):
+        assert torch.equal(a, e)
+    assert [got is d for d, got, _ in used] == [True, True] + [False] * 8 + [True, True]
+    for d in (sd, ad):
+        mine = [got for x, got, _ in used if x is d]
+        for got in mine:
+            assert got.workspace_bytes == d.workspace_bytes and (got is d or got.workspace_tensor is not d.workspace_tensor)
+        held = {got.workspace for got in mine}  # `used` keeps all of them: none was reused
+        assert len(held) == 5
+        assert all(got is d or got.workspace_stream == s for x, got, s in used if x is d)
 
 
 # ---------------------------------------------------------------------------------------------------- key bounds
