@@ -1780,7 +1780,7 @@ __global__ CF_KV_OCC __launch_bounds__(64 * kWavesNarrow) void seam_group_kernel
 //   24 x 32768 (192 units, 256 CUs)  296.5   322.5     32 x 32768, INT8                321.0   315.8
 // A batch padded to one length pays 1.5-5 us (prologue and merge; the loops are alike), one whose mean is below 0.97 of
 // its longest (0.94 at 32 x 4096) gains. Not for
-//   * a single sequence, which cannot be ragged: the splits' smaller workgroups start sooner (17.3 against 24 us at 2003
+//   * a single sequence, which cannot be ragged: the splits' smaller workgroups start sooner (17.6 against 24 us at 2003
 //     tokens);
 //   * tables with room for so few groups that the splits leave less than two chain pairs per wavefront: there is little
 //     to balance, and prologue and merge cost 3 us (20 x 2000 tokens: 26.9 against 29.6 us, 32 x 300: 15.0 against 18.4);

@@ -1,6 +1,6 @@
 // kv_group_body.hpp — one page group through K scores, softmax and P.V by one wavefront (format 4 and INT8 groups of
 // kv_codec_ext.h), shared by the batched decode (kv_batched.hip) and the attention over selected groups of a coded pool
-// (kv_selected_rans.hip). What it does and why stands at the head of kv_batched.hip.
+// (kv_selected.hip). What it does and why stands at the head of kv_batched.hip.
 #pragma once
 
 #include <hip/hip_fp16.h>
@@ -124,7 +124,7 @@ struct VUnit<true> {
 // there).
 // V quads 0..KL-1 do not wait for the V phase in registers: the decode parks them in the wave's LDS area `vl`
 // ([KL][64] words) (RANS), or the V phase loads them again from `raw` (INT8 groups, rare in the launches that use
-// KL > 0). The registers this frees keep the 12-wave kernel free of spills.
+// KL > 0). The registers this frees keep the 12-wave kernel all but free of spills.
 // With kEnds (RANS groups), `ends` receives where the K and V word cursors stopped (words from the K stream's start),
 // so that a caller can check that a self-contained group consumed exactly its words. With kPageVis, `page_vis`
 // tells whether any token of the lane's 16-token page is visible (for callers whose visible tokens are not a prefix
@@ -287,11 +287,12 @@ __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&
   constexpr int kOpExp = RANS ? 24 : 0;
   constexpr int kNone = -(1 << 24);
   // tokens are visible as a prefix of each page, so a page's lane 16 G is visible iff any of its tokens is
-  int ep = (kPageVis ? page_vis : tok_ok) && (!kZeroPages || vs != 0.0f) ? __builtin_amdgcn_frexp_expf(vs) - 15 + kOpExp : kNone;
+  int ep = kNone;
+  if ((kPageVis ? page_vis : tok_ok) && (!kZeroPages || vs != 0.0f)) ep = __builtin_amdgcn_frexp_expf(vs) - 15 + kOpExp;
   int eb = max(max(__builtin_amdgcn_readlane(ep, 0), __builtin_amdgcn_readlane(ep, 16)),
                max(__builtin_amdgcn_readlane(ep, 32), __builtin_amdgcn_readlane(ep, 48)));
-  // kZeroPages: scales far apart: pages whose visible V are all 0 (their scale is 1, or anything) are left out, lest the others' weights
-  // lose their bits to units that nothing needs.
+  // kZeroPages: where scales lie far apart, pages whose visible V are all 0 (their scale is 1, or anything) are left out, lest
+  // the others' weights lose their bits to units that nothing needs.
   if constexpr (kZeroPages) {
     static_assert(KL == 0, "all V quads in registers");
     if (__builtin_amdgcn_ballot_w64(ep < eb - 8 && ep != kNone)) [[unlikely]] {

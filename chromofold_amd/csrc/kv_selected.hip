@@ -7,7 +7,8 @@
 //   weights_out[g] = decay weights_in[g] + sum_h sum_{t in g} p_ht.
 // One pass over the blobs with a running maximum and sum per wavefront; a row's states are joined in LDS or by a second small
 // launch, which also turns the groups' (maximum, sum) pairs into weights. Bound by reading the blobs: 32 x 512 groups of all
-// 8 heads (2.16 GB) at 6.3 TB/s with that launch, 6.7 as one workgroup per row.
+// 8 heads (2.16 GB) at 6.4 TB/s with that launch, 6.7 as one workgroup per row; with 16 query heads per KV head, whose softmax
+// fills all lanes, at 5.5.
 //
 // A wavefront takes one 64-token group (16.4 KB at D = 128) at a time, both products on v_mfma_f32_16x16x32_f16 with the 16
 // rows = query heads, so up to 16 of them cost what one does:
@@ -815,7 +816,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
 // ---- RANS_HYBRID pools: the batched decode's group body (kv_group_body.hpp; at most 4 query heads per KV head), groups of a
 // unit decoded back to back by one wavefront, since a chain may run across them. Bound by the entropy decode, as there: the
 // tables are staged by every workgroup and the memory pipeline restarts at every row. 32 pairs of 512 groups for each of
-// 32 x 8 rows (252 MB) 68 us, all their 512 groups (2.02 GB) 477, 462 without weights (kv_batched.hip 374-396). Two
+// 32 x 8 rows (252 MB) 66 us, all their 512 groups (2.02 GB) 479, 464 without weights (kv_batched.hip 374). Two
 // wavefronts a SIMD: at three the code for raw groups beside the lookups spills (81 and 484 us with 13 registers spilled,
 // 111 and 622 with 58).
 
@@ -1192,12 +1193,13 @@ Plan make_plan(const cf_kv_batched_desc *d, const cf_kv_selection *s) {
   const bool fits = static_cast<uint64_t>(p.slots) * gqa <= kRowStats;  // a row's statistics in LDS
   uint64_t states = 0;
   // us of a call with weights, 8 KV heads, head_dim 128, 4 query heads per KV head unless said, as kSpan / kRow / kSplit:
-  //   32 x 64 of up to 512 groups (list)     60.7 /  45.5 /  52.7      32 x 512 groups            339.9 / 319.6 / 349.2
-  //   1 x 32 groups (list)                   12.6 /  17.7 /  11.6      32 x 8..512 groups         180.9 / 227.4 / 207.9
-  //   16 x 64 groups, 8 query heads          40.9 /  35.7 /  38.8      1 x 512 groups              28.9 / 180.9 /  20.9
-  //   64 x 32 groups                         64.8 /  51.7 /  55.7      1 x 2048 groups             59.2 / 702.1 /  52.1
-  //   64 x 16..125 groups of hd 64           77.6 /  70.3 /  91.1      4 x 2048 groups            162.4 / 718.3 / 170.0
-  //   128 x 32 of 128 groups (list)         110.8 / 103.0 / 106.2      256 x 8..32 groups         157.1 / 142.5 / 145.2
+  //   32 x 64 of up to 512 groups (list)     55.9 /  47.5 /  53.3      32 x 512 groups            336.4 / 320.7 / 356.7
+  //   1 x 32 groups (list)                   13.2 /  19.1 /  12.1      32 x 8..512 groups         179.6 / 229.9 / 209.6
+  //   16 x 64 groups, 8 query heads          40.8 /  36.3 /  36.9      1 x 512 groups              29.3 / 184.2 /  21.9
+  //   64 x 32 groups                         58.9 /  51.8 /  54.8      1 x 2048 groups             60.3 /   -   /  54.3
+  //   64 x 16..125 groups of hd 64           63.9 /  66.3 /  76.7      4 x 2048 groups            163.1 /   -   / 174.0
+  //   128 x 32 of 128 groups (list)         103.1 / 103.6 / 102.0      256 x 8..32 groups         139.0 / 144.4 / 135.3
+  //   16 query heads: 32 x 64 (list)         64.3 /  57.0 /  68.4      32 x 512 groups            394.0 /   -   / 417.3
   // A row to a workgroup where a list makes the rows alike and they fill the chip once, or where they are many and even out
   // by themselves; stretches from 16 slots a resident wavefront on, where its state is small beside them; else splits.
   if (d->codec == CF_KV_CODEC_RANS_HYBRID) p.mode = kCoded;

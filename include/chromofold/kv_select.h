@@ -57,10 +57,11 @@ cf_status cf_kv_key_bounds_async(const float *keys, uint64_t ngroups, const uint
 /* ---- selection -------------------------------------------------------------------------------------------------
  * Score of group g for KV head j of sequence s, over the query heads h of j, with step_h = max |q_h| / 127 and
  * a_h = rint(q_h / step_h) (0 where step_h is 0):
- *   score = max_h(step_h * sum_d max(a_hd * codes[d], -a_hd * codes[D + d])) * scale
+ *   score = max_h(step_h * sum_d (a_hd >= 0 ? a_hd * codes[d] : -a_hd * codes[D + d])) * scale
  * The sum is a whole number below 2^24; each of the two products is rounded to fp32 once, so that scores, and with them the
  * selection, are the same wherever they are computed. It bounds q_h . k over the group's tokens (for the rounded queries;
- * a positive softmax scale is assumed). A unit has the larger score of its groups; a NaN counts as the largest.
+ * a positive softmax scale is assumed). Of a query head, elements that are NaN count as 0; heads with an infinity are passed
+ * over (with no other head the score is -inf * scale). A unit has the larger score of its groups; a NaN counts as the largest.
  *
  * Of the n units that hold a visible token (64 * unit_groups tokens each; visible = min(seq_tokens, query_pos + 1)), the
  * first keep_first and the last keep_last are selected whatever their scores, then the best, min(n, max_units) in all;
@@ -113,7 +114,9 @@ cf_status cf_kv_select_groups_async(const cf_kv_select_desc *desc, void *stream)
  *
  * Pools: INT8 with at most CF_KV_SELECT_MAX_GQA query heads per KV head, RANS_HYBRID (raw groups in it too) with at most 4;
  * more is CF_ERR_UNSUPPORTED. In an INT8 pool a listed group whose header is not an INT8 group of this head_dim makes its
- * row NaN. desc->splits as in the batched call (0 = choose). desc->workspace must hold
+ * row NaN. desc->splits as in the batched call (0 = choose; 1 is the faster choice for many whole rows that the caller knows
+ * to be of one length, INT8, max_groups times query heads per KV head up to 2048: the lengths are device memory, and the
+ * cut that is chosen suits unlike ones). desc->workspace must hold
  * cf_kv_selected_workspace_bytes() bytes, 16-byte aligned. */
 typedef struct cf_kv_selection {
     uint32_t struct_size;
