@@ -176,7 +176,8 @@ cf_status cf_kv_paged_attention_batched_noalloc_async(const cf_kv_batched_desc *
  * merged with each sequence's own groups, which are decoded as by cf_kv_paged_attention_batched_async (desc->codec,
  * desc->splits apply to them). Requirements: head_dim 128; the prefix groups are INT8 blobs (a prefix group of
  * another codec turns the outputs of every sequence into NaN); 1 <= shared_groups <= max_groups. Query positions
- * and sequence lengths mask the prefix like any other tokens. `workspace` must hold
+ * and sequence lengths mask the prefix like any other tokens (but all pages of a prefix group count for the units that its
+ * V is added up in, whichever queries see them). `workspace` must hold
  * cf_kv_cascade_workspace_bytes() bytes; nothing is allocated, nothing synchronises. No counterpart in the
  * reference: its caller is a decode step of many sequences over one long common prefix (e.g. 256 sequences
  * sharing an 8192-token system prompt). */
