@@ -348,8 +348,8 @@ struct RowState {
     int eb = max(max(__builtin_amdgcn_readlane(ep, 0), __builtin_amdgcn_readlane(ep, 4)),
                  max(__builtin_amdgcn_readlane(ep, 8), __builtin_amdgcn_readlane(ep, 12)));
     // Scales far apart: pages whose visible V are all 0 (their scale is 1, or anything) are left out, lest the others'
-    // weights lose their bits to units that nothing needs. (Here, where K's registers
-    // are free: behind the scores the kernels for whole rows spill, 46.3 -> 53.6 us for 32 rows of 64 listed groups.)
+    // weights lose their bits to units that nothing needs. (Here, where K's registers are free: behind the softmax's maximum
+    // the kernels for whole rows spill, 46.3 -> 53.6 us for 248 rows of 64 listed groups.)
     if (__builtin_amdgcn_ballot_w64(ep < eb - 8 && ep != kNone)) [[unlikely]] {
       const int seen = __shfl(static_cast<int>(max(end, page) - page), 4 * b);  // visible tokens of page b, whose V this lane has
       uint32_t any = 0;
@@ -358,7 +358,7 @@ struct RowState {
         uint32_t word = 0;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) word |= w.vw[q * kTiles + i] ^ 0x80808080u;
-        any |= word & (0xFFFFFFFFu >> min(max(32 - 8 * (seen - 4 * q), 0), 31)) & (seen > 4 * q ? ~0u : 0u);  // its visible tokens
+        any |= word & (~0u >> min(max(32 - 8 * (seen - 4 * q), 0), 31)) & (seen > 4 * q ? ~0u : 0u);  // of its visible tokens
       }
       const uint64_t live = __builtin_amdgcn_ballot_w64(any != 0);
       if ((live >> (16 * (n >> 2)) & 0xFFFFu) == 0 && fabsf(vs) < INFINITY) page_vis = false, ep = kNone;
