@@ -130,10 +130,10 @@ struct VUnit<true> {
 // tells whether any token of the lane's 16-token page is visible (for callers whose visible tokens are not a prefix
 // of each page, e.g. behind a causal window); otherwise tok_ok of the page's first lane says it. kStreamRaw: INT8
 // groups' words are read with non-temporal loads (for launches whose groups are each read once). p_out, if given, receives
-// the lane's token's weights exp(score - m_run) of the heads. kZeroPages: pages without any visible V do not set the units
-// (costs the batched decode 3 to 7 %).
+// the lane's token's weights exp(score - m_run) of the heads. kSelected (the attention over selected groups): pages without
+// any visible V do not set the units, which costs the batched decode 3 to 7 %, and groups whose scores are all -inf weigh 0.
 template <int D, int CODEC, int KL, typename WordPtr, typename Hook, bool kEnds = false, bool kPageVis = false,
-          bool kStreamRaw = false, bool kZeroPages = false, bool kCoded>
+          bool kStreamRaw = false, bool kSelected = false, bool kCoded>
 __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&pre)[14], const uint32_t *nlw,
                                            uint32_t (&st)[2], const uint32_t *__restrict__ raw, WordPtr wk,
                                            uint32_t cnt_kv, const uint2 (*__restrict__ s_tab)[kSlots],
@@ -288,12 +288,12 @@ __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&
   constexpr int kNone = -(1 << 24);
   // tokens are visible as a prefix of each page, so a page's lane 16 G is visible iff any of its tokens is
   int ep = kNone;
-  if ((kPageVis ? page_vis : tok_ok) && (!kZeroPages || vs != 0.0f)) ep = __builtin_amdgcn_frexp_expf(vs) - 15 + kOpExp;
+  if ((kPageVis ? page_vis : tok_ok) && (!kSelected || vs != 0.0f)) ep = __builtin_amdgcn_frexp_expf(vs) - 15 + kOpExp;
   int eb = max(max(__builtin_amdgcn_readlane(ep, 0), __builtin_amdgcn_readlane(ep, 16)),
                max(__builtin_amdgcn_readlane(ep, 32), __builtin_amdgcn_readlane(ep, 48)));
-  // kZeroPages: where scales lie far apart, pages whose visible V are all 0 (their scale is 1, or anything) are left out, lest
+  // kSelected: where scales lie far apart, pages whose visible V are all 0 (their scale is 1, or anything) are left out, lest
   // the others' weights lose their bits to units that nothing needs.
-  if constexpr (kZeroPages) {
+  if constexpr (kSelected) {
     static_assert(KL == 0, "all V quads in registers");
     if (__builtin_amdgcn_ballot_w64(ep < eb - 8 && ep != kNone)) [[unlikely]] {
       const uint32_t seen = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(tok_ok) >> (16 * G)) & 0xFFFFu;  // of page G
@@ -325,7 +325,8 @@ __device__ __forceinline__ void group_body(const Hook &after_decode, uint32_t (&
   for (int h = 0; h < kGqa; ++h) {
     const float mn = fmaxf(m_run[h], mx[h]);
     const float a = (m_run[h] == -INFINITY) ? 0.0f : __expf(m_run[h] - mn);
-    pr[h] = tok_ok ? __expf(s[h] - mn) : 0.0f;
+    // kSelected: 0 as long as every score was -inf, where s - mn would be a NaN
+    pr[h] = tok_ok ? __expf(s[h] - (kSelected && mn == -INFINITY ? 0.0f : mn)) : 0.0f;
     l_run[h] = l_run[h] * a + pr[h];
     alpha[h] = ldexpf(a, de);  // ldexp(0, .) = 0 before the first visible token
     m_run[h] = mn;

@@ -816,7 +816,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void span_kernel(SelArgs a) {
 // ---- RANS_HYBRID pools: the batched decode's group body (kv_group_body.hpp; at most 4 query heads per KV head), groups of a
 // unit decoded back to back by one wavefront, since a chain may run across them. Bound by the entropy decode, as there: the
 // tables are staged by every workgroup and the memory pipeline restarts at every row. 32 pairs of 512 groups for each of
-// 32 x 8 rows (252 MB) 66 us, all their 512 groups (2.02 GB) 479, 464 without weights (kv_batched.hip 374). Two
+// 32 x 8 rows (252 MB) 67 us, all their 512 groups (2.02 GB) 482, 468 without weights (kv_batched.hip 374). Two
 // wavefronts a SIMD: at three the code for raw groups beside the lookups spills (81 and 484 us with 13 registers spilled,
 // 111 and 622 with 58).
 
@@ -899,6 +899,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
   uint32_t *buf = s_buf[wave];
   const bool stats = a.s.weights_out != nullptr;
   bool bad = false;  // a list that does not ascend, or a group that continues a chain its unit does not begin
+  bool attended = false;
   // blocks of whole units for the wavefronts; slots are looked up 64 at a time, one a lane
   const uint32_t items = (s1 - s0 + item - 1) / item, pw = (items + W - 1) / W * item;
   const uint32_t w0 = min(s1, s0 + wave * pw), w1 = min(s1, w0 + pw);
@@ -942,6 +943,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
             __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t *>(src + 1024 * k),
                                              (__attribute__((address_space(3))) void *)(buf + 256 * k), 16, 0, 0);
       };
+      attended = true;
       int cur = __builtin_ctzll(todo);
       const uint8_t *blob = blob_at(a, off_l, cur);
       load_header(blob);
@@ -1041,7 +1043,7 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
 #pragma unroll
     for (int h = 0; h < kGqa; ++h) {
       red[h * (D + 2) + D] = broken || l_run[h] != l_run[h] ? __builtin_nanf("") : m_run[h];
-      red[h * (D + 2) + D + 1] = l_run[h];
+      red[h * (D + 2) + D + 1] = attended && m_run[h] == -INFINITY ? 1.0f : l_run[h];  // (see RowState::close)
     }
   }
   __syncthreads();
@@ -1065,6 +1067,9 @@ __global__ __attribute__((amdgpu_waves_per_eu(2, 8))) __launch_bounds__(64 * kWa
         l += rw[D + 1] * f;
         o += rw[dd] * f;
       }
+    else
+#pragma unroll
+      for (int w = 0; w < W; ++w) l += reinterpret_cast<const float *>(s_buf[w])[h * (D + 2) + D + 1];
     a.sums[at * D + i] = o;
     if (dd == 0) a.states[at + h] = float2{nan ? __builtin_nanf("") : m * kLog2e, l};
   }

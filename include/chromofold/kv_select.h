@@ -102,8 +102,7 @@ cf_status cf_kv_select_groups_async(const cf_kv_select_desc *desc, void *stream)
  * lists). Of a row the first min(max_units, n) entries are read, n being its units with a visible token: more cannot be
  * listed. Units without a visible token are passed over; units = NULL takes every group (max_units and unit_groups are then
  * ignored). Rows with nothing to attend are 0; rows whose visible scores are all -inf (as a K scale of +inf can make them) are
- * NaN, as their softmax is; in a RANS_HYBRID pool so may be rows with a group whose scores all are. As in the batched call,
- * with splits = 0 a row's fp32 rounding may depend on the other rows' lengths. As there, V is added up in units of the
+ * NaN, as their softmax is. As in the batched call, with splits = 0 a row's fp32 rounding may depend on the other rows' lengths. As there, V is added up in units of the
  * largest V scale of a group's visible pages, but pages without any visible V other than 0 do not count, whatever their
  * scale: pages with a scale down to 2^-10 of that keep 22 bits, smaller ones fewer, below 2^-31 none (RANS_HYBRID: 2^-18
  * and 2^-39).

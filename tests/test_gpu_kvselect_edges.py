@@ -296,8 +296,8 @@ def test_small_v_beside_absent_pages(dev, monkeypatch, codec, call, gqa, D):
 
 
 @pytest.mark.parametrize("D", [128, 64])
-@pytest.mark.parametrize("gqa", [1, 4, 7, 16])
-def test_scores_of_minus_infinity(dev, monkeypatch, gqa, D):
+@pytest.mark.parametrize("codec, gqa", [(1, 1), (1, 4), (1, 7), (1, 16), (2, 1), (2, 4)])
+def test_scores_of_minus_infinity(dev, monkeypatch, codec, gqa, D):
     """K scales of +inf with products below 0 in all pages (row 0), in some of them (1), in none (2), and in all but with one
     query head whose products are above 0 (3); row 4 has no tokens. Heads whose scores are all -inf are NaN, and so are the
     weights of their groups; others are as if those tokens were not there."""
@@ -306,7 +306,7 @@ def test_scores_of_minus_infinity(dev, monkeypatch, gqa, D):
             k[:] = 0.0
             k[..., 0] = 1.0
     lens = [300, 300, 300, 300, 0]
-    c = cache(monkeypatch, dev, lens, 2, gqa, D, 206, 1, edit)
+    c = cache(monkeypatch, dev, lens, 2, gqa, D, 206, codec, edit, **({"raw_groups": {1: 2}} if codec == 2 else {}))
     gone = {0: range(19), 1: [0, 1, 2, 3, 9, 14], 2: [], 3: range(19)}
     inf = up(dev, np.array([np.inf], np.float32).view(np.uint8))
     for s, pages in gone.items():
@@ -320,7 +320,8 @@ def test_scores_of_minus_infinity(dev, monkeypatch, gqa, D):
         c.q[3, 1, 0] = 0.5  # inf - inf
     left = [[x.copy() for x in c.k[1]], [x.copy() for x in c.v[1]]]
     keep = ~np.isin(np.arange(300) // 16, gone[1])
-    for units, unit in ((None, 1), (np.tile(np.arange(5, dtype=np.uint32), (5, 2, 1)), 1)):
+    listed = np.tile(np.arange(5 if codec == 1 else 3, dtype=np.uint32), (5, 2, 1))
+    for units, unit in ((None, 1), (listed, codec)):  # (a coded pool's chain pairs)
         for splits in (0, 1, 3):
             out, w = c.run(units, unit, weights=None, splits=splits)
             assert np.isnan(out[[0, 3]]).all() and np.isnan(w[[0, 3]]).all(), splits
