@@ -147,6 +147,9 @@ class KeyBounds:
     scales: torch.Tensor
 
 
+_NO_BOUNDS = KeyBounds(None, None)
+
+
 def empty_bounds(seq_count: int, kv_heads: int, max_groups: int, head_dim: int, device="cuda") -> KeyBounds:
     """Records of groups without tokens, to be filled as groups are sealed."""
     return KeyBounds(torch.zeros(seq_count, kv_heads, max_groups, 2 * head_dim, dtype=torch.int8, device=device),
@@ -240,15 +243,14 @@ def select(kvb: kv.BatchedKv, bounds: KeyBounds, queries: torch.Tensor, query_po
     """Fills units int32 [seq_count, kv_heads, max_units] with the units of each row whose bound on the scores of `queries`
     [seq_count, query_heads, D] is largest, the first keep_first and the last keep_last always, ascending, then NO_UNIT."""
     if desc is not None:
-        d = desc
-        _kept(d, (bounds.codes, bounds.scales, kvb.seq_tokens, query_pos, queries, units), (unit_groups, keep_first, keep_last),
-              (1, 1, 1))
+        d, b = desc, bounds if bounds is not None else _NO_BOUNDS
+        _kept(d, (b.codes, b.scales, kvb.seq_tokens, query_pos, queries, units), (unit_groups, keep_first, keep_last), (1, 1, 1))
     else:
         d = select_desc(kvb, bounds, queries, query_pos, units, unit_groups, keep_first, keep_last, stream)
     dev = kvb.group_offsets.device
     s = _raw_stream(dev, stream)
     _call("cf_kv_select_groups_async", dev, s, C.byref(_for_stream(d, cf_kv_select_desc, dev, stream, s)))
-    return units
+    return d.held[5]
 
 
 # ---------------------------------------------------------------------------------------------------- attention
@@ -326,7 +328,7 @@ def _evicted(kvb: kv.BatchedKv, weights: torch.Tensor, out: Evicted | None, boun
             r.codes, r.scales)
 
 
-_NO_BOUNDS, _NO_OUT = KeyBounds(None, None), Evicted(None, None)
+_NO_OUT = Evicted(None, None)
 
 
 def evict_desc(kvb: kv.BatchedKv, weights: torch.Tensor, budget_units: int, out: Evicted | None = None,

@@ -198,15 +198,18 @@ def test_attention_checks_the_pool_and_the_tables(made):
 def test_a_kept_descriptor_takes_its_own_arguments(made):
     k = made
     sd, ad, ed = k.select(), k.attention(), k.evict()
-    k.select(sd)
+    assert k.select(sd) is k.units
+    assert k.select(sd, bounds=None, queries=None, query_pos=None, units=None) is k.units
     k.select(sd, units=k.units.view(S, H, K), unit_groups=2, keep_first=2)
     k.attention(ad)
     k.attention(ad, units=k.units, weights=k.w, weights_out=k.w2, decay=0.9, splits=3, unit_groups=2)
     k.attention(ad, softmax_scale=float(torch.tensor(0.1)))  # the same as float32
+    k.attention(ad, queries=None, output=None, query_pos=None, softmax_scale=None)
     k.evict(ed)
+    k.evict(ed, weights=None, budget_units=None)
     k.evict(ed, out=k.to, bounds=k.b, unit_groups=2, keep_first=0, keep_last=2)
-    assert k.calls == ["cf_kv_select_groups_async"] * 2 + ["cf_kv_paged_attention_selected_async"] * 3 + [
-        "cf_kv_evict_groups_async"] * 2
+    assert k.calls == ["cf_kv_select_groups_async"] * 3 + ["cf_kv_paged_attention_selected_async"] * 4 + [
+        "cf_kv_evict_groups_async"] * 3
 
 
 def test_a_kept_descriptor_refuses_other_arguments(made):
